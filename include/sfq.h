@@ -455,6 +455,73 @@ SFQ_API int sfq_attention_forward(const void* d_q_bf16, int ld_q, const void* d_
                                   void* d_out_bf16, int ld_out, int seq_q, int seq_kv, int heads, int kv_heads,
                                   int head_dim, float scale, void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* ---- a decoding step on the quantized layers ---------------------------------------------------------
+ * For a model that produces one token (or a few) per sequence and step on this library's 4-bit layers. No counterpart in the
+ * reference, whose Linear always goes through the dense bf16 weight or fp4 activations and which keeps no cache. */
+
+/* y[rows, out] = act(x[rows, in] W^T + b) for few rows, without a dense copy of the weight and with bf16 activations: W is what the
+ * stored bytes say (code x group scale x tensor scale, not rounded to bf16), sums are fp32, the result is rounded once. Formats: SFQ_NVFP4
+ * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 32 == 0, block sizes powers of two, of 32 elements at least); no AWQ pre-scale, no ConvRot.
+ * activation: sfq_activation; SFQ_ACT_SWIGLU takes [gate | up] rows (any even out) and writes out / 2 columns. Any number of rows; the
+ * weight is read once for 16 of them. x and the weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
+SFQ_API int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, int rows, int activation, void* d_y_bf16, void* stream);
+
+/* Keys and values of many sequences in pages of `page_size` tokens, 8 bits a value: e4m3 codes, K as [num_pages, kv_heads, page_size, 128]
+ * and V as [num_pages, kv_heads, 128, page_size] (a channel's tokens side by side), each (page, head) with one fp32 scale. d_page_table
+ * [batch, max_pages]: the pages of a sequence in order; entries behind its last page are not read. d_seq_len [batch]: cached tokens of
+ * each sequence, the new ones of this step among them. d_row_start [batch + 1]: the rows of q / k / v / out that are a sequence's new
+ * tokens (none: an empty range); rows behind the last sequence's are left as they were. max_new and max_len are the host's estimates of
+ * the most new tokens and the longest sequence: they size the launch, no result depends on them beyond the order of fp32 sums.
+ * Entries that make no sense are not followed: the tokens they would address are skipped, and sfq_device_status reports 40 (row
+ * starts or a length), 41 (a page outside the pool) or 42 (a rotation position outside the tables). */
+typedef struct sfq_kv_cache {
+  void* d_k;
+  void* d_v;
+  float* d_k_scale; /* [num_pages, kv_heads] */
+  float* d_v_scale;
+  int32_t num_pages;
+  int32_t page_size; /* 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim; /* 128 */
+  const int32_t* d_page_table;
+  const int32_t* d_seq_len;
+  const int32_t* d_row_start;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t max_new;
+  int32_t max_len;
+} sfq_kv_cache;
+
+/* What happens to q and k on the way: RMSNorm over the head (weights bf16 [128], null: none), then a rotation of channel j with
+ * j + rotary_dim / 2 over the first rotary_dim channels (a multiple of 16) by the angles of row `position` of the tables, fp32
+ * [table_rows, rotary_dim / 2] (both null: none). d_position: int32 [rows], null for a token's place in its sequence. All in fp32. */
+typedef struct sfq_rotary {
+  const float* d_cos;
+  const float* d_sin;
+  const int32_t* d_position;
+  int32_t table_rows;
+  int32_t rotary_dim;
+  const void* d_q_norm;
+  const void* d_k_norm;
+  float eps;
+} sfq_rotary;
+
+/* Puts the new tokens' k and v [rows, kv_heads * 128] into their pages and writes q [rows, heads * 128] normed and rotated to d_q_out
+ * (may be d_q itself; heads 0: no q). The scale of a (page, head) is the smallest power of two s (2^-100 at least) with |x| <= 448 s over
+ * the finite values put there so far; a first token in a page starts it anew, a later one can only raise it, and the codes that are there
+ * are then rounded again. Infinities are stored as +-448 s, NaN as NaN. `rotary` may be null. A page that is being written
+ * belongs to one sequence. */
+SFQ_API int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rotary, const void* d_q_bf16, int ld_q, void* d_q_out_bf16,
+                                int ld_q_out, int heads, const void* d_k_bf16, const void* d_v_bf16, int ld_kv, int rows, void* stream);
+
+/* out[rows, heads * 128] = softmax(q K^T scale) V over the cache: the i-th of a sequence's n new tokens sees its first length - n + i + 1
+ * keys; query head h reads kv head h / (heads / kv_heads). scale <= 0 selects 1 / sqrt(128). A row that sees no key is zero; a NaN or +inf
+ * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Slots behind a sequence's length may hold
+ * anything. The workspace is scratch of one call; it needs no initialisation. */
+SFQ_API int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, size_t* out);
+SFQ_API int sfq_kv_cache_attention(const sfq_kv_cache* cache, const void* d_q_bf16, int ld_q, void* d_out_bf16, int ld_out, int heads,
+                                   int rows, float scale, void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- LoRA side branch: y[rows,out] += (x[rows,in] A^T) B^T -------------------------------------------
  * LoraRunner of include/slopfab/cuda/lora.cuh:14-37 (src/cuda/lora.cu:16-93). Factors arrive as fp32 host
  * arrays in model coordinates (LoraFactors, include/slopfab/lora.h:18-23: a[rank,in], b[out_total,rank], the

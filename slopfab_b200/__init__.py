@@ -48,6 +48,19 @@ class SequenceLayout(C.Structure):
                 ("condition_audio_is_explicit", C.c_int32), ("num_audio_rows", C.c_int32), ("num_video_rows", C.c_int32)]
 
 
+class KvCacheDesc(C.Structure):
+    """sfq_kv_cache (include/sfq.h)."""
+    _fields_ = [("d_k", V), ("d_v", V), ("d_k_scale", V), ("d_v_scale", V), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("d_page_table", V), ("d_seq_len", V), ("d_row_start", V),
+                ("batch", C.c_int32), ("max_pages", C.c_int32), ("max_new", C.c_int32), ("max_len", C.c_int32)]
+
+
+class RotaryDesc(C.Structure):
+    """sfq_rotary (include/sfq.h)."""
+    _fields_ = [("d_cos", V), ("d_sin", V), ("d_position", V), ("table_rows", C.c_int32), ("rotary_dim", C.c_int32),
+                ("d_q_norm", V), ("d_k_norm", V), ("eps", F)]
+
+
 class SfqError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"sfq error {code}: {message}")
@@ -129,6 +142,10 @@ def _load() -> C.CDLL:
         "sfq_head_norm_rope": (I, [V, I, V, V, V, I, I, I, C.c_float, V]),
         "sfq_attention_workspace_bytes": (I, [I, I, I, P(SZ)]),
         "sfq_attention_forward": (I, [V, I, V, V, I, V, I, I, I, I, I, I, C.c_float, V, SZ, V]),
+        "sfq_linear_matvec": (I, [P(QuantWeight), V, I, I, V, V]),
+        "sfq_kv_cache_append": (I, [P(KvCacheDesc), P(RotaryDesc), V, I, V, I, I, V, V, I, I, V]),
+        "sfq_kv_cache_attention_workspace_bytes": (I, [P(KvCacheDesc), I, P(SZ)]),
+        "sfq_kv_cache_attention": (I, [P(KvCacheDesc), V, I, V, I, I, I, C.c_float, V, SZ, V]),
         "sfq_lora_create": (I, [P(V)]),
         "sfq_lora_destroy": (None, [V]),
         "sfq_lora_attach": (I, [V, V, V, V, I, I, I, I, I]),
@@ -153,7 +170,8 @@ EXPORTS = ("sfq_last_error sfq_version sfq_quant_weight_init sfq_device_status s
            "sfq_linear_activation_workspace_bytes sfq_linear_forward sfq_linear_prepare "
            "sfq_linear_forward_prepared sfq_linear_nvfp4_forward_static sfq_static_status sfq_build_indices sfq_build_row_timesteps sfq_build_row_timesteps4 sfq_build_adaln_index sfq_weight_row_block sfq_checkpoint_open "
            "sfq_checkpoint_close sfq_checkpoint_count sfq_checkpoint_tensor sfq_checkpoint_metadata sfq_checkpoint_linear sfq_checkpoint_linear_host "
-           "sfq_linear_forward_f32 sfq_adaln_expand sfq_head_norm_rope sfq_attention_workspace_bytes sfq_attention_forward sfq_lora_create sfq_lora_destroy sfq_lora_attach sfq_lora_attach_staged sfq_lora_apply sfq_lora_bytes").split()
+           "sfq_linear_forward_f32 sfq_adaln_expand sfq_head_norm_rope sfq_attention_workspace_bytes sfq_attention_forward "
+           "sfq_linear_matvec sfq_kv_cache_append sfq_kv_cache_attention_workspace_bytes sfq_kv_cache_attention sfq_lora_create sfq_lora_destroy sfq_lora_attach sfq_lora_attach_staged sfq_lora_apply sfq_lora_bytes").split()
 STATIC_SCRATCH_BYTES = 16 * 1024 * 1024
 
 
@@ -195,4 +213,4 @@ def new_weight(**fields) -> QuantWeight:
     return w
 
 
-from .linear import LinearRunner, stream_ptr  # noqa: E402,F401
+from .linear import LinearRunner, linear_matvec, stream_ptr  # noqa: E402,F401

@@ -118,6 +118,29 @@ sfq::GemmArgs to_gemm(const sfq_epilogue* ep, void* y, int M, int N, int K) {
   return g;
 }
 
+sfq::KvCacheView to_cache(const sfq_kv_cache* c, int rows) {
+  if (c == nullptr) throw std::invalid_argument("sfq: null cache descriptor");
+  sfq::KvCacheView v;
+  v.k = static_cast<uint8_t*>(c->d_k);
+  v.v = static_cast<uint8_t*>(c->d_v);
+  v.k_scale = c->d_k_scale;
+  v.v_scale = c->d_v_scale;
+  v.table = c->d_page_table;
+  v.seq_len = c->d_seq_len;
+  v.row_start = c->d_row_start;
+  v.num_pages = c->num_pages;
+  v.kv_heads = c->kv_heads;
+  v.batch = c->batch;
+  v.max_pages = c->max_pages;
+  v.max_new = c->max_new;
+  v.max_len = c->max_len;
+  v.page_shift = -1;
+  for (int s = 4; s <= 8; ++s)
+    if (c->page_size == 1 << s) v.page_shift = s;
+  v.rows = rows;
+  return v;
+}
+
 }  // namespace
 
 // Shared with capi_runner.cu.
@@ -365,6 +388,64 @@ int sfq_attention_forward(const void* d_q_bf16, int ld_q, const void* d_k_bf16, 
     sfq::attention_forward(static_cast<const bf16*>(d_q_bf16), ld_q, static_cast<const bf16*>(d_k_bf16), static_cast<const bf16*>(d_v_bf16),
                            ld_kv, static_cast<bf16*>(d_out_bf16), ld_out, seq_q, seq_kv, heads, kv_heads, head_dim, scale, d_workspace,
                            workspace_bytes, as_stream(stream));
+  });
+}
+int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, int rows, int activation, void* d_y_bf16, void* stream) {
+  return guarded([&] {
+    const sc::QuantWeight q = to_weight(w);
+    if (q.format != sc::QuantFormat::kNVFP4 && q.format != sc::QuantFormat::kNF4) throw std::invalid_argument("matvec: built for NVFP4 and NF4 weights");
+    if (q.pre_quant_scale != nullptr || q.convrot) throw std::invalid_argument("matvec: no AWQ pre-scale and no ConvRot");
+    if (activation != SFQ_ACT_NONE && activation != SFQ_ACT_GELU_TANH && activation != SFQ_ACT_SWIGLU) throw std::invalid_argument("matvec: unknown activation");
+    if (q.bias != nullptr && q.bias_format != sc::QuantFormat::kF32 && q.bias_format != sc::QuantFormat::kBF16)
+      throw std::invalid_argument("matvec: bias must be fp32 or bf16");
+    sfq::MatvecArgs g;
+    g.x = static_cast<const bf16*>(d_x_bf16);
+    g.y = static_cast<bf16*>(d_y_bf16);
+    g.rows = rows, g.out = q.out_features, g.in = q.in_features;
+    g.nf4 = q.format == sc::QuantFormat::kNF4;
+    g.data = static_cast<const uint8_t*>(q.data);
+    g.scale = g.nf4 ? q.nf4_absmax : q.block_scale;
+    g.map = q.nf4_quant_map, g.nested_map = q.nf4_nested_quant_map, g.nested_absmax = q.nf4_nested_absmax;
+    g.offset = q.nf4_nested_offset;
+    g.global_scale = q.global_scale;
+    g.bias = q.bias, g.bias_is_bf16 = q.bias_format == sc::QuantFormat::kBF16;
+    g.act = activation;
+    sfq::linear_matvec(g, q.nf4_block_size, q.nf4_nested_block_size, as_stream(stream));
+  });
+}
+int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rotary, const void* d_q_bf16, int ld_q, void* d_q_out_bf16, int ld_q_out, int heads,
+                        const void* d_k_bf16, const void* d_v_bf16, int ld_kv, int rows, void* stream) {
+  return guarded([&] {
+    sfq::RotaryArgs r;
+    if (rotary != nullptr) {
+      r.cos = rotary->d_cos, r.sin = rotary->d_sin, r.position = rotary->d_position;
+      r.table_rows = rotary->table_rows, r.rotary_dim = rotary->rotary_dim;
+      r.q_norm = static_cast<const bf16*>(rotary->d_q_norm), r.k_norm = static_cast<const bf16*>(rotary->d_k_norm);
+      r.eps = rotary->eps;
+    }
+    sfq::AppendArgs a;
+    a.q = static_cast<const bf16*>(d_q_bf16), a.q_out = static_cast<bf16*>(d_q_out_bf16);
+    a.k = static_cast<const bf16*>(d_k_bf16), a.v = static_cast<const bf16*>(d_v_bf16);
+    a.ld_q = ld_q, a.ld_q_out = ld_q_out, a.ld_kv = ld_kv, a.heads = heads;
+    const sfq::KvCacheView v = to_cache(cache, rows);
+    sfq::kv_append(v, cache->head_dim, r, a, as_stream(stream));
+  });
+}
+int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, size_t* out) {
+  return guarded([&] {
+    if (!out) throw std::invalid_argument("sfq_kv_cache_attention_workspace_bytes: null output");
+    const sfq::KvCacheView v = to_cache(cache, 0);
+    *out = sfq::kv_attention_workspace_bytes(v, cache->head_dim, heads);
+  });
+}
+int sfq_kv_cache_attention(const sfq_kv_cache* cache, const void* d_q_bf16, int ld_q, void* d_out_bf16, int ld_out, int heads, int rows, float scale,
+                           void* d_workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    const sfq::KvCacheView v = to_cache(cache, rows);
+    sfq::KvAttentionArgs a;
+    a.q = static_cast<const bf16*>(d_q_bf16), a.out = static_cast<bf16*>(d_out_bf16);
+    a.ld_q = ld_q, a.ld_out = ld_out, a.heads = heads;
+    sfq::kv_attention(v, cache->head_dim, a, scale, d_workspace, workspace_bytes, as_stream(stream));
   });
 }
 void sfq_test_gemm_variant(int tile_n, int band_m, int max_ctas) { sfq::set_test_gemm_variant(tile_n, band_m, max_ctas); }

@@ -92,6 +92,58 @@ void attention_forward(const __nv_bfloat16* q, int ld_q, const __nv_bfloat16* k,
                        int seq_q, int seq_kv, int heads, int kv_heads, int head_dim, float scale, void* workspace, size_t workspace_bytes,
                        cudaStream_t stream);
 
+// matvec.cu: y = act(W x + b) for few rows, W as stored in 4 bits.
+struct MatvecArgs {
+  const __nv_bfloat16* x = nullptr;  // [rows, in]
+  __nv_bfloat16* y = nullptr;        // [rows, out], out / 2 with SwiGLU
+  int rows = 0, out = 0, in = 0;
+  bool nf4 = false;                  // else NVFP4
+  const uint8_t* data = nullptr;     // two codes a byte, the even element in the high nibble
+  const uint8_t* scale = nullptr;    // NVFP4: e4m3 in the 128x4 tiling; NF4: absmax bytes
+  const float *map = nullptr, *nested_map = nullptr, *nested_absmax = nullptr;  // NF4
+  float offset = 0.0f;
+  int block_shift = 0, nested_shift = 0;
+  float global_scale = 1.0f;
+  const void* bias = nullptr;
+  bool bias_is_bf16 = false;
+  int act = 0;
+};
+void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream_t stream);
+
+// The paged 8-bit cache (kv_append.cu, kv_attention.cu). K [num_pages, kv_heads, page, 128], V [num_pages, kv_heads, 128, page], e4m3;
+// one scale per (page, head).
+struct KvCacheView {
+  uint8_t *k = nullptr, *v = nullptr;
+  float *k_scale = nullptr, *v_scale = nullptr;
+  const int32_t *table = nullptr, *seq_len = nullptr, *row_start = nullptr;
+  int num_pages = 0, page_shift = 0, kv_heads = 0, batch = 0, max_pages = 0, max_new = 0, max_len = 0;
+  int rows = 0;  // of the caller's q, k, v, out
+  int* status = nullptr;
+};
+struct RotaryArgs {
+  const float *cos = nullptr, *sin = nullptr;  // [table_rows, rotary_dim / 2]
+  const int32_t* position = nullptr;           // [rows], null: a token's place in its sequence
+  int table_rows = 0, rotary_dim = 0;
+  const __nv_bfloat16 *q_norm = nullptr, *k_norm = nullptr;
+  float eps = 0.0f;
+};
+struct AppendArgs {
+  const __nv_bfloat16* q = nullptr;
+  __nv_bfloat16* q_out = nullptr;
+  const __nv_bfloat16 *k = nullptr, *v = nullptr;
+  int ld_q = 0, ld_q_out = 0, ld_kv = 0, heads = 0;
+};
+struct KvAttentionArgs {
+  const __nv_bfloat16* q = nullptr;
+  __nv_bfloat16* out = nullptr;
+  int ld_q = 0, ld_out = 0, heads = 0, group = 0;
+  float scale_log2 = 0.0f;
+};
+void kv_check(const KvCacheView& c, int head_dim);
+void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendArgs& g, cudaStream_t stream);
+size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads);
+void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 // LoRA side branch in one launch (lora_kernel.cu): y[rows,out] += bf16(bf16(x a^T) b^T), a [rank,in], b [out,rank]; false,
 // with nothing launched, when rank > 128, a width is no multiple of 8, an operand is not 16-byte aligned, x and y overlap, or two
 // GEMMs are the faster way.

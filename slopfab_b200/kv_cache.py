@@ -1,0 +1,122 @@
+"""ctypes face of the paged 8-bit cache of keys and values (sfq_kv_cache_append, sfq_kv_cache_attention)."""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from . import KvCacheDesc, RotaryDesc, check, lib, ptr, stream_ptr
+from .linear import on_device
+
+HEAD_DIM = 128
+
+
+@dataclass
+class Sequences:
+    """The sequences of a step. page_table int32 [batch, max_pages], seq_len int32 [batch] (new tokens included), row_start int32
+    [batch + 1]; max_new and max_len: the most new tokens of a sequence and the longest sequence, estimates that size the launch."""
+    page_table: torch.Tensor
+    seq_len: torch.Tensor
+    row_start: torch.Tensor
+    max_new: int
+    max_len: int
+
+
+@dataclass
+class Rotary:
+    """What happens to q and k on the way into the cache: head norm (bf16 [128] weights) and rotation (fp32 [table_rows, rotary_dim / 2]
+    tables) at `position` int32 [rows], or at each token's place in its sequence."""
+    cos: torch.Tensor | None = None
+    sin: torch.Tensor | None = None
+    position: torch.Tensor | None = None
+    q_norm: torch.Tensor | None = None
+    k_norm: torch.Tensor | None = None
+    eps: float = 1e-6
+
+    def __post_init__(self):
+        for name, dtype in (("cos", torch.float32), ("sin", torch.float32), ("position", torch.int32), ("q_norm", torch.bfloat16), ("k_norm", torch.bfloat16)):
+            t = getattr(self, name)
+            if t is not None and t.dtype != dtype:
+                raise ValueError(f"{name} must be {dtype}")
+        if (self.cos is None) != (self.sin is None) or (self.cos is not None and (self.cos.dim() != 2 or self.cos.shape != self.sin.shape)):
+            raise ValueError("cos and sin come together, [table_rows, rotary_dim / 2] each")
+        for t in (self.q_norm, self.k_norm):
+            if t is not None and t.shape != (HEAD_DIM,):
+                raise ValueError("norm weights have 128 elements")
+        rows, half = self.cos.shape if self.cos is not None else (0, 0)
+        self.desc = RotaryDesc(ptr(self.cos), ptr(self.sin), ptr(self.position), rows, 2 * half, ptr(self.q_norm), ptr(self.k_norm), self.eps)
+
+
+class KvCache:
+    """Pages of keys and values in e4m3 with one scale per (page, head): k uint8 [pages, kv_heads, page_size, 128], v uint8 [pages,
+    kv_heads, 128, page_size], scales fp32 [pages, kv_heads]. The tensors are the caller's; `KvCache.empty` makes them."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        pages, kv_heads, page_size, dim = k.shape
+        if k.dtype != torch.uint8 or v.dtype != torch.uint8 or v.shape != (pages, kv_heads, dim, page_size):
+            raise ValueError("k must be uint8 [pages, kv_heads, page_size, 128] and v [pages, kv_heads, 128, page_size]")
+        for t in (k_scale, v_scale):
+            if t.dtype != torch.float32 or t.shape != (pages, kv_heads):
+                raise ValueError("scales must be fp32 [pages, kv_heads]")
+        if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
+            raise ValueError("the pools and their scales lie on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.kv_heads, self.device = kv_heads, k.device
+        self._pool = (ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, page_size, kv_heads, dim)
+
+    @staticmethod
+    def empty(pages: int, kv_heads: int, page_size: int = 64, device="cuda") -> "KvCache":
+        k = torch.zeros((pages, kv_heads, page_size, HEAD_DIM), dtype=torch.uint8, device=device)
+        v = torch.zeros((pages, kv_heads, HEAD_DIM, page_size), dtype=torch.uint8, device=device)
+        return KvCache(k, v, *(torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)))
+
+    def _desc(self, s: Sequences) -> KvCacheDesc:
+        t = s.page_table
+        if t.dtype != torch.int32 or s.seq_len.dtype != torch.int32 or s.row_start.dtype != torch.int32:
+            raise ValueError("page_table, seq_len and row_start must be int32")
+        batch, max_pages = t.shape
+        if s.seq_len.shape != (batch,) or s.row_start.shape != (batch + 1,):
+            raise ValueError("seq_len has an entry per sequence, row_start one more")
+        if not t.device == s.seq_len.device == s.row_start.device == self.device:
+            raise ValueError("the sequences' tensors lie on the cache's device")
+        return KvCacheDesc(*self._pool, ptr(t), ptr(s.seq_len), ptr(s.row_start), batch, max_pages, s.max_new, s.max_len)
+
+    def _rows(self, name: str, t: torch.Tensor, cols: int) -> int:
+        if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != cols or t.stride(1) != 1 or t.device != self.device:
+            raise ValueError(f"{name} must be bf16 [rows, {cols}] with contiguous rows, on the cache's device")
+        return t.stride(0)
+
+    def append(self, s: Sequences, qkv: torch.Tensor, heads: int, q_out: torch.Tensor | None = None, rotary: Rotary | None = None) -> torch.Tensor:
+        """Stores k and v of the fused projection qkv [rows, (heads + 2 kv_heads) * 128] and returns q, normed and rotated
+        (q_out [rows, heads * 128]; pass a view of qkv's first columns to have it in place)."""
+        ld, rows = self._rows("qkv", qkv, (heads + 2 * self.kv_heads) * HEAD_DIM), qkv.shape[0]
+        if q_out is None:
+            q_out = torch.empty((rows, heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+        ld_out = self._rows("q_out", q_out, heads * HEAD_DIM)
+        if q_out.shape[0] != rows:
+            raise ValueError("q_out has as many rows as qkv")
+        if rotary is not None and rotary.position is not None and rotary.position.shape != (rows,):
+            raise ValueError("position has an entry per row")
+        q = qkv.data_ptr()
+        k = q + heads * HEAD_DIM * 2
+        with on_device(self.device):
+            check(lib.sfq_kv_cache_append(C.byref(self._desc(s)), C.byref(rotary.desc) if rotary is not None else None, q, ld, q_out.data_ptr(), ld_out,
+                                          heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, stream_ptr()))
+        return q_out
+
+    def attention(self, s: Sequences, q: torch.Tensor, heads: int, out: torch.Tensor | None = None, scale: float = 0.0) -> torch.Tensor:
+        """softmax(q K^T scale) V of the new tokens' q [rows, heads * 128] over the cache, causal among them; scale 0 means 1 / sqrt(128).
+        The workspace is the call's own, so that calls on several streams and captured graphs share none."""
+        ld, rows = self._rows("q", q, heads * HEAD_DIM), q.shape[0]
+        if out is None:
+            out = torch.empty((rows, heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
+        ld_out = self._rows("out", out, heads * HEAD_DIM)
+        if out.shape[0] != rows:
+            raise ValueError("out has as many rows as q")
+        with on_device(self.device):
+            desc, n = self._desc(s), C.c_size_t()
+            check(lib.sfq_kv_cache_attention_workspace_bytes(C.byref(desc), heads, C.byref(n)))
+            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+            check(lib.sfq_kv_cache_attention(C.byref(desc), q.data_ptr(), ld, out.data_ptr(), ld_out, heads, rows, scale, ws.data_ptr(), n.value, stream_ptr()))
+        return out

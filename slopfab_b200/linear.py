@@ -7,16 +7,43 @@ a caller-visible torch uint8 tensor, grown to the high-water mark like the refer
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
 
-from . import COMPUTE_BF16, QuantWeight, check, lib, ptr
+from . import ACT_NONE, ACT_SWIGLU, COMPUTE_BF16, QuantWeight, check, lib, ptr
 
 
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def on_device(device: torch.device):
+    """Makes the device of a call's tensors current for it, at no cost where it is already."""
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not on {device}")
+    return _SAME if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_SAME = contextlib.nullcontext()
+
+
+def linear_matvec(w: QuantWeight, x: torch.Tensor, y: torch.Tensor | None = None, activation: int = ACT_NONE) -> torch.Tensor:
+    """y = act(x W^T + b) for the few rows of a decoding step, the NVFP4 or NF4 weight read as stored (sfq_linear_matvec).
+    x: bf16 [rows, in]; y: bf16 [rows, out], out / 2 columns with ACT_SWIGLU. Runs on x's device and its current stream."""
+    cols = w.out_features // 2 if activation == ACT_SWIGLU else w.out_features
+    if x.dim() != 2 or x.shape[1] != w.in_features or x.dtype != torch.bfloat16:
+        raise ValueError(f"x must be bf16 [rows, {w.in_features}]")
+    rows, device = x.shape[0], x.device
+    if y is None:
+        y = torch.empty((rows, cols), dtype=torch.bfloat16, device=device)
+    elif y.shape != (rows, cols) or y.dtype != torch.bfloat16 or y.device != device:
+        raise ValueError(f"y must be bf16 [{rows}, {cols}] on x's device")
+    with on_device(device):
+        check(lib.sfq_linear_matvec(C.byref(w), ptr(x), rows, activation, ptr(y), stream_ptr()))
+    return y
 
 
 class LinearRunner:

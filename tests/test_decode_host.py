@@ -1,0 +1,137 @@
+"""Refusals of the decoding-step entry points: each is made on the host before anything is launched, so no GPU is needed."""
+import ctypes as C
+
+import pytest
+import torch
+
+import slopfab_b200 as sfq
+from slopfab_b200.kv_cache import KvCache, Rotary, Sequences
+
+A = 1 << 20  # stands for an aligned device address; nothing here is dereferenced
+
+
+def _weight(**over):
+    f = dict(format=sfq.NVFP4, data=A, block_scale=A, out_features=256, in_features=128)
+    f.update(over)
+    return sfq.new_weight(**f)
+
+
+def _nf4(**over):
+    f = dict(format=sfq.NF4, data=A, nf4_absmax=A, nf4_quant_map=A, nf4_nested_quant_map=A, nf4_nested_absmax=A, out_features=34, in_features=96)
+    f.update(over)
+    return sfq.new_weight(**f)
+
+
+def _matvec(w, x=A, rows=2, act=0, y=2 * A):
+    return sfq.lib.sfq_linear_matvec(C.byref(w) if w is not None else None, x, rows, act, y, None)
+
+
+@pytest.mark.parametrize("w,text", [
+    (lambda: _weight(format=sfq.W4A8), b"NVFP4 and NF4"), (lambda: _weight(format=sfq.BF16), b"NVFP4 and NF4"),
+    (lambda: _weight(pre_quant_scale=A), b"pre-scale"), (lambda: _weight(convrot=1), b"ConvRot"),
+    (lambda: _weight(out_features=200), b"% 128"), (lambda: _weight(in_features=96), b"% 64"), (lambda: _weight(out_features=0), b"positive"),
+    (lambda: _weight(data=None), b"null"), (lambda: _weight(block_scale=None), b"block_scale"), (lambda: _weight(data=A + 8), b"aligned"),
+    (lambda: _weight(block_scale=A + 2), b"aligned"), (lambda: _weight(bias=A, bias_format=sfq.F16), b"bias"),
+    (lambda: _nf4(in_features=80), b"% 32"), (lambda: _nf4(nf4_block_size=48), b"powers of two"), (lambda: _nf4(nf4_block_size=16), b"powers of two"),
+    (lambda: _nf4(nf4_nested_block_size=100), b"powers of two"), (lambda: _nf4(nf4_absmax=None), b"double-quant"),
+])
+def test_matvec_refuses_weights(w, text):
+    assert _matvec(w()) == sfq.ERR_INVALID_ARGUMENT
+    assert text in sfq.lib.sfq_last_error()
+
+
+def test_matvec_refuses_calls():
+    assert _matvec(None) == sfq.ERR_INVALID_ARGUMENT
+    assert _matvec(_weight(), act=7) == sfq.ERR_INVALID_ARGUMENT
+    assert _matvec(_nf4(out_features=33), act=sfq.ACT_SWIGLU) == sfq.ERR_INVALID_ARGUMENT and b"even" in sfq.lib.sfq_last_error()
+    for x, y in ((None, A), (A, None), (A + 2, 2 * A), (A, 2 * A + 1), (A, A), (A, A + 2 * 2 * 128 - 2), (A + 2 * 2 * 256 - 16, A)):
+        assert _matvec(_weight(), x=x, y=y) == sfq.ERR_INVALID_ARGUMENT, (x, y)
+    assert _matvec(_weight(), rows=0, x=None, y=None) == sfq.OK and _matvec(_weight(), rows=-3) == sfq.OK  # no-ops
+
+
+def _cache(**over):
+    f = dict(d_k=A, d_v=A, d_k_scale=A, d_v_scale=A, num_pages=7, page_size=64, kv_heads=2, head_dim=128, d_page_table=A, d_seq_len=A, d_row_start=A,
+             batch=3, max_pages=4, max_new=1, max_len=200)
+    f.update(over)
+    return sfq.KvCacheDesc(**f)
+
+
+BAD_CACHES = [dict(head_dim=64), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(num_pages=0), dict(kv_heads=0), dict(batch=0),
+              dict(max_pages=0), dict(max_new=0), dict(max_len=0), dict(d_k=None), dict(d_v=None), dict(d_k_scale=None), dict(d_v_scale=None),
+              dict(d_page_table=None), dict(d_seq_len=None), dict(d_row_start=None), dict(d_k=A + 8), dict(d_v=A + 8), dict(kv_heads=40000)]
+
+
+def _append(c, rotary=None, q=A, ld_q=512, q_out=A, ld_q_out=512, heads=4, k=A, v=A, ld_kv=256, rows=3):
+    return sfq.lib.sfq_kv_cache_append(C.byref(c) if c is not None else None, C.byref(rotary) if rotary is not None else None, q, ld_q, q_out, ld_q_out,
+                                       heads, k, v, ld_kv, rows, None)
+
+
+def _attend(c, q=A, ld_q=512, out=2 * A, ld_out=512, heads=4, rows=3, ws=A, ws_bytes=1 << 40):
+    return sfq.lib.sfq_kv_cache_attention(C.byref(c) if c is not None else None, q, ld_q, out, ld_out, heads, rows, 0.0, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("over", BAD_CACHES)
+def test_bad_caches_are_refused(over):
+    assert _append(_cache(**over)) == sfq.ERR_INVALID_ARGUMENT
+    assert _attend(_cache(**over)) == sfq.ERR_INVALID_ARGUMENT
+    n = C.c_size_t()
+    assert sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache(**over)), 4, C.byref(n)) == sfq.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(q_out=None), dict(k=None), dict(v=None), dict(heads=-1), dict(ld_q=504), dict(ld_q=516),
+                                  dict(ld_q_out=504), dict(ld_kv=248), dict(ld_kv=260), dict(q=A + 8), dict(q_out=A + 8), dict(k=A + 8), dict(v=A + 2)])
+def test_append_refuses_operands(over):
+    assert _append(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("over", [dict(d_sin=None), dict(d_cos=None), dict(rotary_dim=0), dict(rotary_dim=24), dict(rotary_dim=144), dict(table_rows=0),
+                                  dict(d_cos=A + 4), dict(d_q_norm=A + 2), dict(d_k_norm=A + 2)])
+def test_append_refuses_rotations(over):
+    f = dict(d_cos=A, d_sin=A, table_rows=5, rotary_dim=96, d_q_norm=A, d_k_norm=A, eps=1e-6)
+    f.update(over)
+    assert _append(_cache(), rotary=sfq.RotaryDesc(**f)) == sfq.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(ws=None), dict(ws_bytes=0), dict(heads=0), dict(heads=3), dict(ld_q=504),
+                                  dict(ld_out=516), dict(out=A), dict(q=A + 8), dict(out=2 * A + 2)])
+def test_attention_refuses_operands(over):
+    assert _attend(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
+
+
+def test_no_rows_is_a_no_op_and_null_descriptors_are_refused():
+    assert _append(_cache(), rows=0, q=None, k=None) == sfq.OK and _attend(_cache(), rows=0, q=None) == sfq.OK
+    assert _append(None) == sfq.ERR_INVALID_ARGUMENT and _attend(None) == sfq.ERR_INVALID_ARGUMENT
+    assert sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache()), 4, None) == sfq.ERR_INVALID_ARGUMENT
+
+
+def test_python_faces_refuse_what_does_not_fit():
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    cache = KvCache.empty(5, 2, 64, device="cpu")
+    seqs = Sequences(i32(3, 4), i32(3), i32(4), 1, 100)
+    qkv = torch.zeros((3, 8 * 128), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA device"):  # there is no CPU path
+        cache.append(seqs, qkv, 4)
+    with pytest.raises(ValueError, match="CUDA device"):
+        cache.attention(seqs, qkv[:, :512], 4)
+    with pytest.raises(ValueError, match="CUDA device"):
+        sfq.linear_matvec(_weight(), torch.zeros((1, 128), dtype=torch.bfloat16))
+    for bad in (qkv.float(), qkv[:, :-128], qkv[0], qkv.t().contiguous().t()):
+        with pytest.raises(ValueError):
+            cache.append(seqs, bad, 4)
+    with pytest.raises(ValueError):
+        cache.append(seqs, qkv, 4, q_out=torch.zeros((2, 512), dtype=torch.bfloat16))
+    for bad in (torch.zeros((1, 64), dtype=torch.bfloat16), torch.zeros((1, 128)), torch.zeros(128, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            sfq.linear_matvec(_weight(), bad)
+    with pytest.raises(ValueError):
+        sfq.linear_matvec(_weight(), torch.zeros((1, 128), dtype=torch.bfloat16), torch.zeros((1, 128), dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        KvCache(cache.k, cache.k, cache.k_scale, cache.v_scale)
+    with pytest.raises(ValueError):
+        KvCache(cache.k, cache.v, cache.k_scale[:4], cache.v_scale)
+    with pytest.raises(ValueError):
+        Rotary(cos=torch.zeros((4, 48)))
+    with pytest.raises(ValueError):
+        Rotary(q_norm=torch.ones(64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        Rotary(torch.zeros((4, 48)), torch.zeros((4, 48)), position=torch.zeros(3))
