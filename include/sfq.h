@@ -461,7 +461,8 @@ SFQ_API int sfq_attention_forward(const void* d_q_bf16, int ld_q, const void* d_
 
 /* y[rows, out] = act(x[rows, in] W^T + b) for few rows, without a dense copy of the weight and with bf16 activations: W is what the
  * stored bytes say (code x group scale x tensor scale, not rounded to bf16), sums are fp32, the result is rounded once. Formats: SFQ_NVFP4
- * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 32 == 0, block sizes powers of two, of 32 elements at least); no AWQ pre-scale, no ConvRot.
+ * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 64 == 0, block sizes powers of two, of 64 elements at least; the 16
+ * table entries are rounded to fp16); no AWQ pre-scale, no ConvRot.
  * activation: sfq_activation; SFQ_ACT_SWIGLU takes [gate | up] rows (any even out) and writes out / 2 columns. Any number of rows; the
  * weight is read once for 16 of them. x and the weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
 SFQ_API int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, int rows, int activation, void* d_y_bf16, void* stream);

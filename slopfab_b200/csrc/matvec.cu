@@ -1,10 +1,21 @@
 // y = act(W x + b) for few rows of x, W as stored in 4 bits with group scales (NVFP4, NF4).
 //
 // Bound by the weight's bytes: N K / 2 codes and N K / 16 (NVFP4) or about N K / 64 (NF4) scale bytes are read once, whatever the
-// number of rows. Weight values are used as the bytes define them (code x group scale x tensor scale, without the rounding to
-// bf16 that the dense form has), sums are fp32, and the result is rounded once, behind bias and activation.
+// number of rows. At the measured copy rate an SM is sent 41 weights a clock, and its integer pipe does 64 operations a clock, so a
+// weight may cost about one and a half instructions. That decides the arithmetic:
+//   - products on mma.sync m16n8k16 (fp16 operands, fp32 sums): 16 weight rows are its M, up to 8 rows of x its N. One MMA takes 256
+//     weights; tcgen05 would need whole tiles of decoded weights in shared memory first.
+//   - NVFP4: a byte becomes two fp16 by one conversion instruction, times its group's scale by one packed product. 2 + 4 significant bits
+//     and 2^-10 .. 2688 are exact in fp16. bf16 weights would need five integer instructions a pair.
+//   - NF4: a byte is looked up as two fp16 (the table's entries rounded by 2^-11) in a table of all 256 bytes that has a copy for each
+//     lane's bank; the absmax of 64 elements scales the fp32 sum of their four MMAs.
+//   - x becomes fp16 times a power of two for each row, exactly: see stage_x.
+// A CTA takes 16 MT weight rows and its eight warps take turns along K in steps of 128, each with its own ring of asynchronous copies;
+// their sums meet in shared memory in a fixed order.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 
@@ -18,8 +29,68 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kWarps = 8;
-constexpr int kMostRows = 16;  // rows of x in one launch
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kMostRows = 16;      // rows of x in one launch
+constexpr int kStep = 128;         // elements of K a warp takes at a time
+constexpr int kTableBytes = 65536; // NF4: entry of byte b for lane l at b * 256 + l * 4
+
+struct Plan {
+  int slab = 0;        // elements of K whose x is in shared memory at a time, a multiple of kWarps * kStep
+  int absmax_off = 0;  // byte offsets into shared memory
+  int x_off = 0;
+  int ring_off = 0;
+  int groups = 0;      // NF4: 64-element groups of a row
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The four bytes of w as pairs of fp16, low nibble in the low half, each pair times the scale pair s.
+__device__ __forceinline__ void decode_e2m1(uint32_t w, uint32_t s, uint32_t (&v)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t.reg .b32 t;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 t, b0;\n\tmul.f16x2 %0, t, %5;\n\tcvt.rn.f16x2.e2m1x2 t, b1;\n\tmul.f16x2 %1, t, %5;\n\t"
+      "cvt.rn.f16x2.e2m1x2 t, b2;\n\tmul.f16x2 %2, t, %5;\n\tcvt.rn.f16x2.e2m1x2 t, b3;\n\tmul.f16x2 %3, t, %5;\n\t}"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+      : "r"(w), "r"(s));
+}
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {
+  uint32_t v;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(v) : "h"(uint16_t(two)));
+  return v;
+}
 
 __device__ __forceinline__ float activated(float z, float up, int act) {
   if (act == SFQ_ACT_GELU_TANH) return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z)));
@@ -27,61 +98,313 @@ __device__ __forceinline__ float activated(float z, float up, int act) {
   return z;
 }
 
-// One warp per output column (a pair of weight rows for SwiGLU), lanes along K.
-template <bool NF4>
-__global__ void __launch_bounds__(kWarps * 32) matvec_kernel(MatvecArgs g) {
+// The weight row that is row i of 16-row tile t. NVFP4 keeps the scales of rows n, n + 32, n + 64, n + 96 side by side, so a tile takes four
+// neighbours from each of the four quarters of 128 rows, whose scales for 64 elements are 64 bytes in a piece (with SwiGLU two quarters
+// of gate rows, and the same of up rows). Rows past the end of an NF4 weight stand for its last one and are not stored.
+template <bool NF4> __device__ __forceinline__ int weight_row(int t, int i, int out, bool swiglu) {
+  if (swiglu) {
+    const int j = i & 7, half = out >> 1;
+    const int col = NF4 ? min(t * 8 + j, half - 1) : (t >> 3) * 64 + (j >> 2) * 32 + (t & 7) * 4 + (j & 3);
+    return (i < 8 ? 0 : half) + col;
+  }
+  return NF4 ? min(t * 16 + i, out - 1) : (t >> 3) * 128 + (i >> 2) * 32 + (t & 7) * 4 + (i & 3);
+}
+
+// fp16 is as good as bf16 for x where every element of a row lies within 32 binades: times a power of two, its eight significant bits fit
+// (as subnormals at the lower end). The first attempt takes 2^6, good for zeros and 2^-23 <= |x| < 2^10. Rows with others are sent
+// through the weight again, with the exponent of their own largest element and, where they span more than 32 binades, in bands of 32
+// binades, the smallest first. Infinities and NaN go with the topmost band.
+constexpr int kFixedExponent = 8;  // the largest exponent of the first attempt's range is one above it
+
+// One element of x for band `band` below row exponent e: times 2^(14 - e + 32 band), 0 where it belongs to another band.
+__device__ __forceinline__ float banded(float f, int e, int band) {
+  const uint32_t u = __float_as_uint(f) & 0x7FFFFFFFu;
+  if (u >= 0x7F800000u) return band == 0 ? f : 0.0f;
+  if (u == 0) return 0.0f;
+  const int mine = u >= 0x800000u ? int(u >> 23) - 127 : 31 - __clz(int(u)) - 149;
+  const int which = (e - mine) >> 5;
+  if (which != band) return 0.0f;
+  return ldexpf(f, 14 - e + 32 * band);
+}
+
+template <bool NF4, int NT, int MT>
+__global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) {
+  constexpr int D = MT == 1 ? 4 : MT == 2 ? 3 : 2;            // ring stages
+  constexpr int kStage = MT * 1024 + (NF4 ? 0 : MT * 128);    // codes [MT][16 rows][64 bytes], scales [MT][2 slabs][16 rows][4 bytes]
+  constexpr int kCols = NT * 8;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint32_t flags;
+  __shared__ int row_e[kMostRows], row_low[kMostRows];
+  __shared__ float nested_map[NF4 ? 256 : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
+  const bool swiglu = g.act == SFQ_ACT_SWIGLU;
+  const int steps = (g.in + kStep - 1) / kStep;
+  const uint32_t base = smem_u32(smem);
+  const uint32_t ring = base + p.ring_off + warp * D * kStage;
+  const int tile0 = blockIdx.x * MT;
   grid_dependency_release();
+
+  const uint8_t* src[MT][2];  // this lane's 16 bytes of rows gq and gq + 8 of each tile, step 0
+  const uint8_t* scale_src[MT];  // NVFP4: four scales of row lane % 16, slab lane / 16
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) src[m][h] = g.data + size_t(weight_row<NF4>(tile0 + m, gq + 8 * h, g.out, swiglu)) * (g.in / 2) + q * 16;
+    if constexpr (!NF4) scale_src[m] = g.scale + nvfp4_scale_offset(weight_row<NF4>(tile0 + m, lane & 15, g.out, swiglu), (lane >> 4) * 4, g.in / 16);
+  }
+  // Step s of K into slot `slot` of this warp's ring; elements past the end are zeros.
+  auto fetch = [&](int s, int slot) {
+    if (s < steps) {
+      const uint32_t to = ring + slot * kStage;
+      const bool live = s * kStep + q * 32 < g.in;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = gq + 8 * h;
+          const int unit = NF4 ? q ^ (row & 2) : q;  // NF4 is read in 8-byte pieces of four rows at a time
+          cp_async16(to + m * 1024 + row * 64 + unit * 16, live ? src[m][h] + size_t(s) * 64 : g.data, live);
+        }
+        if constexpr (!NF4) {
+          const bool there = s * kStep + (lane >> 4) * 64 < g.in;
+          cp_async4(to + MT * 1024 + m * 128 + lane * 4, there ? scale_src[m] + size_t(s) * 1024 : g.scale, there);
+        }
+      }
+    }
+    cp_commit();
+  };
+
+  float acc[MT][NT][4];
   grid_dependency_wait();
-  __shared__ float map[16];
-  if (threadIdx.x < 16) map[threadIdx.x] = NF4 ? g.map[threadIdx.x] : e2m1_decode(threadIdx.x);
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const int col = blockIdx.x * kWarps + int(threadIdx.x >> 5);
-  const int cols = g.act == SFQ_ACT_SWIGLU ? g.out / 2 : g.out;
-  if (col >= cols) return;
-  const int halves = g.act == SFQ_ACT_SWIGLU ? 2 : 1;
-  float sum[2][kMostRows];
-  for (int h = 0; h < 2; ++h)
-    for (int r = 0; r < kMostRows; ++r) sum[h][r] = 0.0f;
-  for (int h = 0; h < halves; ++h) {
-    const int n = col + h * cols;
-    const uint8_t* w = g.data + size_t(n) * (g.in / 2);
-    for (int k = lane * 16; k < g.in; k += 512) {
-      float scale;
-      if (NF4) {
-        const size_t block = (size_t(n) * g.in + k) >> g.block_shift;
-        scale = fmaf(g.nested_map[g.scale[block]], g.nested_absmax[block >> g.nested_shift], g.offset);
-      } else {
-        scale = e4m3_decode(g.scale[nvfp4_scale_offset(n, k / 16, g.in / 16)]);
-      }
-      const uint2 raw = *reinterpret_cast<const uint2*>(w + k / 2);
-      float v[16];
+  for (int i = 0; i < D - 1; ++i) fetch(warp + i * kWarps, i);
+  if (threadIdx.x == 0) flags = 0;
+  if constexpr (NF4) {
+    // the table: thread b builds the entry of byte b, odd element (low nibble) in the low half, and its 32 copies
+    const uint32_t b = threadIdx.x;
+    const __half2 pair = __floats2half2_rn(g.map[b & 15], g.map[b >> 4]);
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(&pair);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t byte = ((i < 4 ? raw.x : raw.y) >> (8 * (i & 3))) & 0xFFu;
-        v[2 * i] = map[byte >> 4] * scale;
-        v[2 * i + 1] = map[byte & 15u] * scale;
-      }
-#pragma unroll
-      for (int r = 0; r < kMostRows; ++r) {
-        if (r >= g.rows) break;
-        const __nv_bfloat16* x = g.x + size_t(r) * g.in + k;
-        for (int i = 0; i < 16; ++i) sum[h][r] = fmaf(v[i], __bfloat162float(x[i]), sum[h][r]);
-      }
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(smem + b * 256 + ((i + b) & 7) * 16) = make_uint4(v, v, v, v);
+    nested_map[b] = g.nested_map[b];
+    for (int r = 0; r < MT * 16; ++r) {
+      const size_t first = (size_t(weight_row<NF4>(tile0 + (r >> 4), r & 15, g.out, swiglu)) * g.in);
+      for (int i = threadIdx.x; i < p.groups; i += kThreads) smem[p.absmax_off + r * p.groups + i] = g.scale[(first + size_t(i) * 64) >> g.block_shift];
     }
   }
+  const float* const nested_absmax = g.nested_absmax;
+  size_t group0[MT][2];  // NF4: element index of the lane's rows
+  if constexpr (NF4) {
 #pragma unroll
-  for (int r = 0; r < kMostRows; ++r) {
-    if (r >= g.rows) break;
-    float z[2];
-    for (int h = 0; h < halves; ++h) {
-      float s = sum[h][r];
-      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-      const int n = col + h * cols;
-      const float b = g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[n]) : static_cast<const float*>(g.bias)[n];
-      z[h] = fmaf(s, g.global_scale, b);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) group0[m][h] = size_t(weight_row<NF4>(tile0 + m, gq + 8 * h, g.out, swiglu)) * g.in;
+  }
+
+  // x [rows, k0 .. k0 + slab) as fp16: 16 bytes of eight elements, pairs with the odd element in the low half, at unit
+  // ((step * 4 + piece) * rows + row) * 4 + lane % 4, which is the order in which the MMAs' lanes read them.
+  auto stage_x = [&](int k0, int band) {  // band < 0: the first attempt
+    const int units = min(p.slab, steps * kStep - k0) / 8;
+    const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x3400), __ushort_as_bfloat16(0x3400));  // 2^-23
+    const __nv_bfloat162 zero = __halves2bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
+    uint32_t low = 0;
+    __nv_bfloat162 top = zero;
+    for (int r = 0; r < g.rows; ++r) {
+      const __nv_bfloat16* row = g.x + size_t(r) * g.in + k0;
+      for (int k8 = threadIdx.x; k8 < units; k8 += kThreads) {
+        const uint4 raw = k0 + k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(row + k8 * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float even = __uint_as_float(w[i] << 16), odd = __uint_as_float(w[i] & 0xFFFF0000u);
+          if (band < 0) {
+            const uint32_t mag = w[i] & 0x7FFF7FFFu;
+            const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&mag);
+            low |= __hlt2_mask(a, least) & __hgt2_mask(a, zero);
+            top = __hmax2(top, a);
+            even *= 64.0f, odd *= 64.0f;
+          } else {
+            even = banded(even, row_e[r], band), odd = banded(odd, row_e[r], band);
+          }
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(even), "f"(odd));
+        }
+        const int step = k8 >> 4;
+        const int piece = NF4 ? ((k8 >> 3) & 1) * 2 + (k8 & 1) : k8 & 3, quarter = NF4 ? (k8 >> 1) & 3 : (k8 >> 2) & 3;
+        *reinterpret_cast<uint4*>(smem + p.x_off + (((step * 4 + piece) * g.rows + r) * 4 + quarter) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
     }
-    if (lane == 0) g.y[size_t(r) * cols + col] = __float2bfloat16(activated(z[0], z[halves - 1], g.act));
+    if (band < 0 && (low != 0 || fmaxf(__low2float(top), __high2float(top)) >= 1024.0f)) flags = 1;
+  };
+
+  auto multiply = [&](int s, int slot, int local) {  // step s, whose x is step `local` of the slab
+    const uint32_t from = ring + slot * kStage;
+    const uint32_t xs = base + p.x_off + (local * 4 * g.rows * 4 + lane) * 16;
+    if constexpr (!NF4) {
+      uint4 w[MT][2];
+      uint32_t sc[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = gq + 8 * h;
+          w[m][h] = lds128(from + m * 1024 + row * 64 + q * 16);
+          sc[m][h] = e4m3_pair(lds16(from + MT * 1024 + m * 128 + (q >> 1) * 64 + row * 4 + (q & 1) * 2));
+        }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 xv[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) xv[n] = gq + 8 * n < g.rows ? lds128(xs + (j * g.rows + 8 * n) * 64) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t word = j == 0 ? w[m][h].x : j == 1 ? w[m][h].y : j == 2 ? w[m][h].z : w[m][h].w;
+            decode_e2m1(word, __byte_perm(sc[m][h], 0, j < 2 ? 0x1010 : 0x3232), a[h]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_f16(acc[m][n], a[0][0], a[1][0], a[0][1], a[1][1], xv[n].x, xv[n].y);
+            mma_f16(acc[m][n], a[0][2], a[1][2], a[0][3], a[1][3], xv[n].z, xv[n].w);
+          }
+        }
+      }
+    } else {
+      const uint32_t lane4 = lane * 4;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int group = s * 2 + c;
+        if (group >= p.groups) break;
+        uint4 xv[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) xv[n][j] = gq + 8 * n < g.rows ? lds128(xs + ((c * 2 + j) * g.rows + 8 * n) * 64) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint2 w[2];
+          float scale[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = gq + 8 * h;
+            w[h] = lds64(from + m * 1024 + row * 64 + ((c * 2 + (q >> 1)) ^ (row & 2)) * 16 + (q & 1) * 8);
+            const size_t block = (group0[m][h] + size_t(group) * 64) >> g.block_shift;
+            scale[h] = fmaf(nested_map[smem[p.absmax_off + (m * 16 + row) * p.groups + group]], nested_absmax[block >> g.nested_shift], g.offset);
+          }
+          float d[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t word = j == 0 ? w[h].x : w[h].y;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) a[h][i] = lds32(base + __byte_perm(word, lane4, 0x7704 | (i << 4)));
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_f16(d[n], a[0][0], a[1][0], a[0][1], a[1][1], xv[n][j].x, xv[n][j].y);
+              mma_f16(d[n], a[0][2], a[1][2], a[0][3], a[1][3], xv[n][j].z, xv[n][j].w);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[m][n][0] = fmaf(d[n][0], scale[0], acc[m][n][0]), acc[m][n][1] = fmaf(d[n][1], scale[0], acc[m][n][1]);
+            acc[m][n][2] = fmaf(d[n][2], scale[1], acc[m][n][2]), acc[m][n][3] = fmaf(d[n][3], scale[1], acc[m][n][3]);
+          }
+        }
+      }
+    }
+  };
+
+  // Once along K for one band of x. The first D - 1 steps of this warp are under way.
+  auto pass = [&](int band) {
+    int slot = 0;
+    for (int k0 = 0; k0 < steps * kStep; k0 += p.slab) {
+      if (k0 > 0) __syncthreads();  // the slab in front has been read
+      stage_x(k0, band);
+      __syncthreads();
+      const int end = min(steps, (k0 + p.slab) / kStep);
+      for (int s = k0 / kStep + warp; s < end; s += kWarps) {
+        fetch(s + (D - 1) * kWarps, slot == 0 ? D - 1 : slot - 1);
+        cp_wait<D - 1>();
+        __syncwarp();
+        multiply(s, slot, s - k0 / kStep);
+        __syncwarp();
+        slot = slot == D - 1 ? 0 : slot + 1;
+      }
+    }
+  };
+  auto clear = [&](float by) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][n][e] = by == 0.0f ? 0.0f : acc[m][n][e] * by;
+  };
+
+  if (threadIdx.x < kMostRows) row_e[threadIdx.x] = kFixedExponent;
+  __syncthreads();  // flags, and the table
+  clear(0.0f);
+  pass(-1);
+  __syncthreads();
+  if (flags != 0) {
+    // Each row's largest exponent and lowest band, over its finite elements that are not zero.
+    for (int r = warp; r < g.rows; r += kWarps) {
+      int most = -1000, least = 1000;
+      for (int k = lane; k < g.in; k += 32) {
+        const uint32_t u = __float_as_uint(__bfloat162float(g.x[size_t(r) * g.in + k])) & 0x7FFFFFFFu;
+        if (u == 0 || u >= 0x7F800000u) continue;
+        const int e = u >= 0x800000u ? int(u >> 23) - 127 : 31 - __clz(int(u)) - 149;
+        most = max(most, e), least = min(least, e);
+      }
+      most = __reduce_max_sync(0xffffffffu, most), least = __reduce_min_sync(0xffffffffu, least);
+      if (lane == 0) row_e[r] = most == -1000 ? 0 : most, row_low[r] = most == -1000 ? 0 : (most - least) >> 5;
+    }
+    __syncthreads();
+    int bands = 0;
+    for (int r = 0; r < g.rows; ++r) bands = max(bands, row_low[r]);
+    clear(0.0f);
+    for (int band = bands; band >= 0; --band) {
+      cp_wait<0>();
+      __syncthreads();
+      for (int i = 0; i < D - 1; ++i) fetch(warp + i * kWarps, i);
+      if (band < bands) clear(0x1p-32f);
+      pass(band);
+    }
+    __syncthreads();
+  }
+  cp_wait<0>();
+
+  // The warps' sums, in shared memory [warp][16 MT rows][kCols + 1] over what is no longer needed.
+  constexpr int kPitch = kCols + 1;
+  float* part = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[(warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)] = acc[m][n][e];
+  __syncthreads();
+  const int cols = swiglu ? g.out / 2 : g.out;
+  const int per_tile = swiglu ? 8 : 16;
+  for (int i = threadIdx.x; i < MT * per_tile * g.rows; i += kThreads) {
+    const int r = i / (MT * per_tile), local = i - r * (MT * per_tile), m = local / per_tile, j = local - m * per_tile;
+    const int n = weight_row<NF4>(tile0 + m, j, g.out, swiglu);
+    if (NF4 ? (tile0 + m) * per_tile + j >= cols : n >= cols) continue;
+    float z[2];
+    for (int h = 0; h < (swiglu ? 2 : 1); ++h) {
+      float s = 0.0f;
+      for (int w = 0; w < kWarps; ++w) s += part[(w * MT * 16 + m * 16 + j + 8 * h) * kPitch + r];
+      const int at = n + h * cols;
+      const float b = g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
+      z[h] = ldexpf(s * g.global_scale, row_e[r] - 14) + b;
+    }
+    g.y[size_t(r) * cols + n] = __float2bfloat16(activated(z[0], swiglu ? z[1] : 0.0f, g.act));
   }
 }
 
@@ -93,6 +416,44 @@ int log2_of(int v) {
 bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+template <bool NF4, int NT, int MT> void launch(const MatvecArgs& g, cudaStream_t stream) {
+  constexpr int D = MT == 1 ? 4 : MT == 2 ? 3 : 2;
+  const bool swiglu = g.act == SFQ_ACT_SWIGLU;
+  const int tiles = NF4 ? ((swiglu ? g.out / 2 : g.out) + (swiglu ? 7 : 15)) / (swiglu ? 8 : 16) : g.out / 16;
+  Plan p;
+  int at = NF4 ? kTableBytes : 0;
+  p.absmax_off = at;
+  if (NF4) p.groups = g.in / 64, at += (MT * 16 * p.groups + 15) / 16 * 16;
+  p.x_off = at;
+  constexpr int kTurn = kWarps * kStep;
+  const int whole = (g.in + kTurn - 1) / kTurn * kTurn;
+  p.slab = std::max(kTurn, std::min(whole, 81920 / (2 * g.rows) / kTurn * kTurn));
+  at += std::min(p.slab, (g.in + kStep - 1) / kStep * kStep) * g.rows * 2;
+  p.ring_off = at;
+  at += kWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
+  at = std::max(at, kWarps * MT * 16 * (NT * 8 + 1) * 4);
+  if (at > 230000) throw std::invalid_argument("matvec: in_features too large");
+  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT>), size_t(at), "matvec");
+  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT>, dim3((tiles + MT - 1) / MT), dim3(kThreads), size_t(at), stream, g, p);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("matvec: launch failed: ") + cudaGetErrorString(e));
+}
+
+template <bool NF4> void launch_rows(const MatvecArgs& g, cudaStream_t stream) {
+  const int tiles = NF4 ? (g.out + 15) / 16 : g.out / 16;
+  int mt = g.rows <= 2 ? 1 : g.rows <= 4 ? 2 : 4;
+  while (mt > 1 && tiles < mt * device_sm_count()) mt /= 2;
+  while (NF4 && mt > 1 && mt * g.in > 131072) mt /= 2;  // the absmax bytes of the tiles' rows
+  if (g.rows <= 8) {
+    if (mt == 1) launch<NF4, 1, 1>(g, stream);
+    else if (mt == 2) launch<NF4, 1, 2>(g, stream);
+    else launch<NF4, 1, 4>(g, stream);
+  } else {
+    if (mt == 1) launch<NF4, 2, 1>(g, stream);
+    else if (mt == 2) launch<NF4, 2, 2>(g, stream);
+    else launch<NF4, 2, 4>(g, stream);
+  }
+}
+
 }  // namespace
 
 void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream_t stream) {
@@ -101,8 +462,8 @@ void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream
   if (!g.x || !g.y || !g.data) throw std::invalid_argument("matvec: null operand");
   if (g.nf4) {
     if (!g.scale || !g.map || !g.nested_map || !g.nested_absmax) throw std::invalid_argument("matvec: nf4 weight without complete double-quant state");
-    if (!power_of_two(nf4_block) || nf4_block < 32 || !power_of_two(nf4_nested_block)) throw std::invalid_argument("matvec: nf4 blocks must be powers of two, of 32 elements at least");
-    if (g.in % 32 != 0) throw std::invalid_argument("matvec: nf4 needs in_features % 32 == 0");
+    if (!power_of_two(nf4_block) || nf4_block < 64 || !power_of_two(nf4_nested_block)) throw std::invalid_argument("matvec: nf4 blocks must be powers of two, of 64 elements at least");
+    if (g.in % 64 != 0) throw std::invalid_argument("matvec: nf4 needs in_features % 64 == 0");
     g.block_shift = log2_of(nf4_block), g.nested_shift = log2_of(nf4_nested_block);
     g.global_scale = 1.0f;
   } else {
@@ -120,12 +481,13 @@ void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream
   const int rows = g.rows;
   for (int r = 0; r < rows; r += kMostRows) {
     MatvecArgs part = g;
-    part.rows = rows - r < kMostRows ? rows - r : kMostRows;
+    part.rows = std::min(rows - r, kMostRows);
     part.x = g.x + size_t(r) * g.in;
     part.y = g.y + size_t(r) * cols;
-    const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, g.nf4 ? matvec_kernel<true> : matvec_kernel<false>, dim3((cols + kWarps - 1) / kWarps),
-                                            dim3(kWarps * 32), 0, stream, part);
-    if (e != cudaSuccess) throw std::runtime_error(std::string("matvec: launch failed: ") + cudaGetErrorString(e));
+    if (g.nf4)
+      launch_rows<true>(part, stream);
+    else
+      launch_rows<false>(part, stream);
   }
 }
 

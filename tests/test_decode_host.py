@@ -17,7 +17,7 @@ def _weight(**over):
 
 
 def _nf4(**over):
-    f = dict(format=sfq.NF4, data=A, nf4_absmax=A, nf4_quant_map=A, nf4_nested_quant_map=A, nf4_nested_absmax=A, out_features=34, in_features=96)
+    f = dict(format=sfq.NF4, data=A, nf4_absmax=A, nf4_quant_map=A, nf4_nested_quant_map=A, nf4_nested_absmax=A, out_features=34, in_features=192)
     f.update(over)
     return sfq.new_weight(**f)
 
@@ -32,7 +32,7 @@ def _matvec(w, x=A, rows=2, act=0, y=2 * A):
     (lambda: _weight(out_features=200), b"% 128"), (lambda: _weight(in_features=96), b"% 64"), (lambda: _weight(out_features=0), b"positive"),
     (lambda: _weight(data=None), b"null"), (lambda: _weight(block_scale=None), b"block_scale"), (lambda: _weight(data=A + 8), b"aligned"),
     (lambda: _weight(block_scale=A + 2), b"aligned"), (lambda: _weight(bias=A, bias_format=sfq.F16), b"bias"),
-    (lambda: _nf4(in_features=80), b"% 32"), (lambda: _nf4(nf4_block_size=48), b"powers of two"), (lambda: _nf4(nf4_block_size=16), b"powers of two"),
+    (lambda: _nf4(in_features=96), b"% 64"), (lambda: _nf4(nf4_block_size=48), b"powers of two"), (lambda: _nf4(nf4_block_size=32), b"powers of two"),
     (lambda: _nf4(nf4_nested_block_size=100), b"powers of two"), (lambda: _nf4(nf4_absmax=None), b"double-quant"),
 ])
 def test_matvec_refuses_weights(w, text):

@@ -91,13 +91,13 @@ def check(w, x, act="none"):
 
 
 @pytest.mark.parametrize("fmt,n,k", [("nvfp4", 128, 64), ("nvfp4", 256, 192), ("nvfp4", 384, 1024), ("nvfp4", 1152, 4160), ("nvfp4", 640, 13824),
-                                     ("nf4", 2, 32), ("nf4", 34, 96), ("nf4", 7, 224), ("nf4", 250, 1056), ("nf4", 1025, 4128), ("nf4", 514, 13824)])
+                                     ("nf4", 2, 64), ("nf4", 34, 128), ("nf4", 7, 192), ("nf4", 250, 1088), ("nf4", 1025, 4160), ("nf4", 514, 13824)])
 @pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 16, 17, 37])
 def test_shapes(fmt, n, k, rows):
     check(Weight(fmt, n, k, n + k), draw_x(rows, k, rows))
 
 
-@pytest.mark.parametrize("fmt,n,k", [("nvfp4", 384, 704), ("nvfp4", 128, 5120), ("nf4", 42, 160), ("nf4", 1026, 2048)])
+@pytest.mark.parametrize("fmt,n,k", [("nvfp4", 384, 704), ("nvfp4", 128, 5120), ("nf4", 42, 192), ("nf4", 1026, 2048)])
 @pytest.mark.parametrize("rows", [1, 5, 12])
 @pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
 @pytest.mark.parametrize("bias", [None, torch.float32, torch.bfloat16])
@@ -105,9 +105,9 @@ def test_activations_and_bias(fmt, n, k, rows, act, bias):
     check(Weight(fmt, n, k, n, bias), draw_x(rows, k, rows) * (0.05 if fmt == "nvfp4" else 0.5), act)
 
 
-@pytest.mark.parametrize("block,nested", [(32, 1), (64, 256), (128, 4), (4096, 256)])
+@pytest.mark.parametrize("block,nested", [(64, 1), (64, 256), (128, 4), (4096, 256)])
 def test_nf4_block_sizes(block, nested):
-    check(Weight("nf4", 130, 416, block, None, block, nested), draw_x(3, 416, 1))
+    check(Weight("nf4", 130, 448, block, None, block, nested), draw_x(3, 448, 1))
 
 
 def test_a_packed_weight_against_the_dense_arm():
