@@ -10,7 +10,8 @@
 //   - NF4: a byte is looked up as two fp16 (the table's entries rounded by 2^-11) in a table of all 256 bytes that has a copy for each
 //     lane's bank; the absmax of 64 elements scales the fp32 sum of their four MMAs.
 //   - x becomes fp16 times a power of two for each row, exactly: see stage_x.
-// A CTA takes 16 MT weight rows and its eight warps take turns along K in steps of 128, each with its own ring of asynchronous copies;
+// CTAs stay for the whole launch, so that x is made fp16 once per SM. Each has two teams of eight warps; a team takes 16 MT weight rows at
+// a time, its warps take turns along K in steps of 128, each with its own ring of asynchronous copies that runs on into the next rows, and
 // their sums meet in shared memory in a fixed order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -29,19 +30,18 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kTeams = 2, kTeamWarps = 8, kThreads = kTeams * kTeamWarps * 32;
+constexpr size_t kMostSmem = 229376;  // dynamic; the kernel has about 2 KB of its own
 constexpr int kMostRows = 16;      // rows of x in one launch
 constexpr int kStep = 128;         // elements of K a warp takes at a time
 constexpr int kTableBytes = 65536; // NF4: entry of byte b for lane l at b * 256 + l * 4
 
 struct Plan {
-  int slab = 0;        // elements of K whose x is in shared memory at a time, a multiple of kWarps * kStep
-  int absmax_off = 0;  // byte offsets into shared memory
-  int x_off = 0;
-  int ring_off = 0;
-  int groups = 0;      // NF4: 64-element groups of a row
+  int units = 0;  // groups of MT tiles of 16 weight rows
+  int ring_off = 0, part_off = 0, x_off = 0;  // byte offsets into shared memory
 };
 
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
@@ -127,91 +127,98 @@ __device__ __forceinline__ float banded(float f, int e, int band) {
   return ldexpf(f, 14 - e + 32 * band);
 }
 
-template <bool NF4, int NT, int MT>
-__global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) {
-  constexpr int D = MT == 1 ? 4 : MT == 2 ? 3 : 2;            // ring stages
-  constexpr int kStage = MT * 1024 + (NF4 ? 0 : MT * 128);    // codes [MT][16 rows][64 bytes], scales [MT][2 slabs][16 rows][4 bytes]
-  constexpr int kCols = NT * 8;
-  extern __shared__ __align__(1024) uint8_t smem[];
+template <bool NF4, int NT, int MT, int D>
+__global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_kernel(MatvecArgs g, Plan p) {
+  constexpr int kStage = MT * 1024 + (NF4 ? 0 : MT * 128);  // codes [MT][16 rows][64 bytes], scales [MT][2 slabs][16 rows][4 bytes]
+  constexpr int kPitch = NT * 8 + 1;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t flags;
   __shared__ int row_e[kMostRows], row_low[kMostRows];
   __shared__ float nested_map[NF4 ? 256 : 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
+  const int warp = (threadIdx.x >> 5) % kTeamWarps, team = threadIdx.x / (kTeamWarps * 32), lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
   const bool swiglu = g.act == SFQ_ACT_SWIGLU;
   const int steps = (g.in + kStep - 1) / kStep;
   const uint32_t base = smem_u32(smem);
-  const uint32_t ring = base + p.ring_off + warp * D * kStage;
-  const int tile0 = blockIdx.x * MT;
+  const uint32_t ring = base + p.ring_off + (threadIdx.x >> 5) * D * kStage;
+  const int first_unit = blockIdx.x * kTeams + team, all_teams = gridDim.x * kTeams;
   grid_dependency_release();
 
-  const uint8_t* src[MT][2];  // this lane's 16 bytes of rows gq and gq + 8 of each tile, step 0
+  // The copies under way: the next one is step `fs` of unit `fu`.
+  int fu, fs;
+  const uint8_t* src[MT][2];     // this lane's 16 bytes of rows gq and gq + 8 of each tile
   const uint8_t* scale_src[MT];  // NVFP4: four scales of row lane % 16, slab lane / 16
+  auto seek = [&](int unit) {
+    fu = unit, fs = warp;
+    if (unit >= p.units) return;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) src[m][h] = g.data + size_t(weight_row<NF4>(tile0 + m, gq + 8 * h, g.out, swiglu)) * (g.in / 2) + q * 16;
-    if constexpr (!NF4) scale_src[m] = g.scale + nvfp4_scale_offset(weight_row<NF4>(tile0 + m, lane & 15, g.out, swiglu), (lane >> 4) * 4, g.in / 16);
-  }
-  // Step s of K into slot `slot` of this warp's ring; elements past the end are zeros.
-  auto fetch = [&](int s, int slot) {
-    if (s < steps) {
+      for (int h = 0; h < 2; ++h)
+        src[m][h] = g.data + size_t(weight_row<NF4>(unit * MT + m, gq + 8 * h, g.out, swiglu)) * (g.in / 2) + q * 16 + size_t(warp) * (kStep / 2);
+      if constexpr (!NF4)
+        scale_src[m] = g.scale + nvfp4_scale_offset(weight_row<NF4>(unit * MT + m, lane & 15, g.out, swiglu), (lane >> 4) * 4, g.in / 16) + size_t(warp) * (kStep * 8);
+    }
+  };
+  auto fetch = [&](int slot, int end_unit) {  // elements past the end of a row are zeros
+    if (fs < steps && fu < end_unit) {
       const uint32_t to = ring + slot * kStage;
-      const bool live = s * kStep + q * 32 < g.in;
+      const bool live = fs * kStep + q * 32 < g.in;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int row = gq + 8 * h;
           const int unit = NF4 ? q ^ (row & 2) : q;  // NF4 is read in 8-byte pieces of four rows at a time
-          cp_async16(to + m * 1024 + row * 64 + unit * 16, live ? src[m][h] + size_t(s) * 64 : g.data, live);
+          cp_async16(to + m * 1024 + row * 64 + unit * 16, live ? src[m][h] : g.data, live);
+          src[m][h] += kTeamWarps * kStep / 2;
         }
         if constexpr (!NF4) {
-          const bool there = s * kStep + (lane >> 4) * 64 < g.in;
-          cp_async4(to + MT * 1024 + m * 128 + lane * 4, there ? scale_src[m] + size_t(s) * 1024 : g.scale, there);
+          const bool there = fs * kStep + (lane >> 4) * 64 < g.in;
+          cp_async4(to + MT * 1024 + m * 128 + lane * 4, there ? scale_src[m] : g.scale, there);
+          scale_src[m] += kTeamWarps * kStep * 8;
         }
       }
+      fs += kTeamWarps;
+      if (fs >= steps) seek(fu + all_teams);
     }
     cp_commit();
   };
+  // NF4: lane l holds the absmax of row l / 2, group l % 2 of a step: its byte and its nested scale, fetched a step ahead.
+  uint32_t absmax_byte[MT];
+  float absmax_outer[MT];
+  auto fetch_absmax = [&](int unit, int s) {
+    if constexpr (NF4) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int group = min(s * 2 + (lane & 1), g.in / 64 - 1);
+        const size_t block = (size_t(weight_row<true>(unit * MT + m, lane >> 1, g.out, swiglu)) * g.in + size_t(group) * 64) >> g.block_shift;
+        absmax_byte[m] = g.scale[block], absmax_outer[m] = g.nested_absmax[block >> g.nested_shift];
+      }
+    }
+  };
 
   float acc[MT][NT][4];
-  grid_dependency_wait();
-  for (int i = 0; i < D - 1; ++i) fetch(warp + i * kWarps, i);
-  if (threadIdx.x == 0) flags = 0;
-  if constexpr (NF4) {
-    // the table: thread b builds the entry of byte b, odd element (low nibble) in the low half, and its 32 copies
-    const uint32_t b = threadIdx.x;
-    const __half2 pair = __floats2half2_rn(g.map[b & 15], g.map[b >> 4]);
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(&pair);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(smem + b * 256 + ((i + b) & 7) * 16) = make_uint4(v, v, v, v);
-    nested_map[b] = g.nested_map[b];
-    for (int r = 0; r < MT * 16; ++r) {
-      const size_t first = (size_t(weight_row<NF4>(tile0 + (r >> 4), r & 15, g.out, swiglu)) * g.in);
-      for (int i = threadIdx.x; i < p.groups; i += kThreads) smem[p.absmax_off + r * p.groups + i] = g.scale[(first + size_t(i) * 64) >> g.block_shift];
-    }
-  }
-  const float* const nested_absmax = g.nested_absmax;
-  size_t group0[MT][2];  // NF4: element index of the lane's rows
-  if constexpr (NF4) {
+  auto scale_sums = [&](float by) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) group0[m][h] = size_t(weight_row<NF4>(tile0 + m, gq + 8 * h, g.out, swiglu)) * g.in;
-  }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][n][e] = by == 0.0f ? 0.0f : acc[m][n][e] * by;
+  };
 
-  // x [rows, k0 .. k0 + slab) as fp16: 16 bytes of eight elements, pairs with the odd element in the low half, at unit
+  // x [rows, in] as fp16: 16 bytes of eight elements, pairs with the odd element in the low half, at unit
   // ((step * 4 + piece) * rows + row) * 4 + lane % 4, which is the order in which the MMAs' lanes read them.
-  auto stage_x = [&](int k0, int band) {  // band < 0: the first attempt
-    const int units = min(p.slab, steps * kStep - k0) / 8;
+  auto stage_x = [&](int band) {  // band < 0: the first attempt
+    const int units = steps * kStep / 8;
     const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x3400), __ushort_as_bfloat16(0x3400));  // 2^-23
     const __nv_bfloat162 zero = __halves2bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
     uint32_t low = 0;
     __nv_bfloat162 top = zero;
     for (int r = 0; r < g.rows; ++r) {
-      const __nv_bfloat16* row = g.x + size_t(r) * g.in + k0;
+      const __nv_bfloat16* row = g.x + size_t(r) * g.in;
       for (int k8 = threadIdx.x; k8 < units; k8 += kThreads) {
-        const uint4 raw = k0 + k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(row + k8 * 8) : make_uint4(0, 0, 0, 0);
+        const uint4 raw = k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(row + k8 * 8) : make_uint4(0, 0, 0, 0);
         const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
         uint32_t o[4];
 #pragma unroll
@@ -236,9 +243,9 @@ __global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) 
     if (band < 0 && (low != 0 || fmaxf(__low2float(top), __high2float(top)) >= 1024.0f)) flags = 1;
   };
 
-  auto multiply = [&](int s, int slot, int local) {  // step s, whose x is step `local` of the slab
+  auto multiply = [&](int s, int slot) {
     const uint32_t from = ring + slot * kStage;
-    const uint32_t xs = base + p.x_off + (local * 4 * g.rows * 4 + lane) * 16;
+    const uint32_t xs = base + p.x_off + (s * 4 * g.rows * 4 + lane) * 16;
     if constexpr (!NF4) {
       uint4 w[MT][2];
       uint32_t sc[MT][2];
@@ -272,10 +279,12 @@ __global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) 
       }
     } else {
       const uint32_t lane4 = lane * 4;
+      float absmax[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) absmax[m] = fmaf(nested_map[absmax_byte[m]], absmax_outer[m], g.offset);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int group = s * 2 + c;
-        if (group >= p.groups) break;
+        if (s * 2 + c >= g.in / 64) break;
         uint4 xv[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -289,8 +298,7 @@ __global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) 
           for (int h = 0; h < 2; ++h) {
             const int row = gq + 8 * h;
             w[h] = lds64(from + m * 1024 + row * 64 + ((c * 2 + (q >> 1)) ^ (row & 2)) * 16 + (q & 1) * 8);
-            const size_t block = (group0[m][h] + size_t(group) * 64) >> g.block_shift;
-            scale[h] = fmaf(nested_map[smem[p.absmax_off + (m * 16 + row) * p.groups + group]], nested_absmax[block >> g.nested_shift], g.offset);
+            scale[h] = __shfl_sync(0xffffffffu, absmax[m], row * 2 + c);
           }
           float d[NT][4];
 #pragma unroll
@@ -320,41 +328,79 @@ __global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) 
     }
   };
 
-  // Once along K for one band of x. The first D - 1 steps of this warp are under way.
-  auto pass = [&](int band) {
-    int slot = 0;
-    for (int k0 = 0; k0 < steps * kStep; k0 += p.slab) {
-      if (k0 > 0) __syncthreads();  // the slab in front has been read
-      stage_x(k0, band);
-      __syncthreads();
-      const int end = min(steps, (k0 + p.slab) / kStep);
-      for (int s = k0 / kStep + warp; s < end; s += kWarps) {
-        fetch(s + (D - 1) * kWarps, slot == 0 ? D - 1 : slot - 1);
-        cp_wait<D - 1>();
-        __syncwarp();
-        multiply(s, slot, s - k0 / kStep);
-        __syncwarp();
-        slot = slot == D - 1 ? 0 : slot + 1;
-      }
+  // This warp's steps of a unit. Their first D - 1 copies are under way, and go on with the units up to end_unit.
+  int slot = 0;
+  auto walk = [&](int unit, int end_unit) {
+    for (int s = warp; s < steps; s += kTeamWarps) {
+      fetch(slot == 0 ? D - 1 : slot - 1, end_unit);
+      cp_wait<D - 1>();
+      __syncwarp();
+      multiply(s, slot);
+      if (s + kTeamWarps < steps)
+        fetch_absmax(unit, s + kTeamWarps);
+      else if (unit + all_teams < end_unit)
+        fetch_absmax(unit + all_teams, warp);
+      __syncwarp();
+      slot = slot == D - 1 ? 0 : slot + 1;
     }
   };
-  auto clear = [&](float by) {
+  auto start = [&](int unit, int end_unit) {
+    slot = 0;
+    seek(unit);
+    for (int i = 0; i < D - 1; ++i) fetch(i, end_unit);
+    if (unit < end_unit && warp < steps) fetch_absmax(unit, warp);
+  };
+
+  // The team's sums of a unit, added in the order of its warps, finished and stored.
+  float* const part = reinterpret_cast<float*>(smem + p.part_off) + team * kTeamWarps * MT * 16 * kPitch;
+  const int cols = swiglu ? g.out / 2 : g.out;
+  auto finish = [&](int unit) {
+    named_barrier(team + 1, kTeamWarps * 32);  // the sums of the unit in front have been read
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][n][e] = by == 0.0f ? 0.0f : acc[m][n][e] * by;
+        for (int e = 0; e < 4; ++e) part[(warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)] = acc[m][n][e];
+    named_barrier(team + 1, kTeamWarps * 32);
+    const int per_tile = swiglu ? 8 : 16;
+    for (int i = warp * 32 + lane; i < MT * per_tile * g.rows; i += kTeamWarps * 32) {
+      const int r = i / (MT * per_tile), local = i - r * (MT * per_tile), m = local / per_tile, j = local - m * per_tile;
+      const int n = weight_row<NF4>(unit * MT + m, j, g.out, swiglu);
+      if (NF4 && (unit * MT + m) * per_tile + j >= cols) continue;
+      float z[2] = {0.0f, 0.0f};
+      for (int h = 0; h < (swiglu ? 2 : 1); ++h) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kTeamWarps; ++w) s += part[(w * MT * 16 + m * 16 + j + 8 * h) * kPitch + r];
+        const int at = n + h * cols;
+        const float b = g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
+        z[h] = ldexpf(s * g.global_scale, row_e[r] - 14) + b;
+      }
+      g.y[size_t(r) * cols + n] = __float2bfloat16(activated(z[0], z[1], g.act));
+    }
   };
 
+  grid_dependency_wait();
+  start(first_unit, p.units);
+  if (threadIdx.x == 0) flags = 0;
   if (threadIdx.x < kMostRows) row_e[threadIdx.x] = kFixedExponent;
-  __syncthreads();  // flags, and the table
-  clear(0.0f);
-  pass(-1);
+  if constexpr (NF4) {
+    // the table: two threads build the entry of a byte, odd element (low nibble) in the low half, and its 32 copies
+    const uint32_t b = threadIdx.x & 255;
+    const __half2 pair = __floats2half2_rn(g.map[b & 15], g.map[b >> 4]);
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(&pair);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(smem + b * 256 + ((i * 2 + (threadIdx.x >> 8) + b) & 7) * 16) = make_uint4(v, v, v, v);
+    if (threadIdx.x < 256) nested_map[b] = g.nested_map[b];
+  }
+  __syncthreads();  // flags
+  stage_x(-1);
   __syncthreads();
+  int bands = 0;
   if (flags != 0) {
     // Each row's largest exponent and lowest band, over its finite elements that are not zero.
-    for (int r = warp; r < g.rows; r += kWarps) {
+    for (int r = threadIdx.x >> 5; r < g.rows; r += kThreads / 32) {
       int most = -1000, least = 1000;
       for (int k = lane; k < g.in; k += 32) {
         const uint32_t u = __float_as_uint(__bfloat162float(g.x[size_t(r) * g.in + k])) & 0x7FFFFFFFu;
@@ -366,46 +412,35 @@ __global__ void __launch_bounds__(kThreads) matvec_kernel(MatvecArgs g, Plan p) 
       if (lane == 0) row_e[r] = most == -1000 ? 0 : most, row_low[r] = most == -1000 ? 0 : (most - least) >> 5;
     }
     __syncthreads();
-    int bands = 0;
     for (int r = 0; r < g.rows; ++r) bands = max(bands, row_low[r]);
-    clear(0.0f);
-    for (int band = bands; band >= 0; --band) {
-      cp_wait<0>();
+    if (bands == 0) {
+      stage_x(0);
       __syncthreads();
-      for (int i = 0; i < D - 1; ++i) fetch(warp + i * kWarps, i);
-      if (band < bands) clear(0x1p-32f);
-      pass(band);
     }
-    __syncthreads();
+  }
+  if (bands == 0) {
+    for (int unit = first_unit; unit < p.units; unit += all_teams) {
+      scale_sums(0.0f);
+      walk(unit, p.units);
+      finish(unit);
+    }
+  } else {
+    for (int first = blockIdx.x * kTeams; first < p.units; first += all_teams) {  // the teams in step, since x changes under them
+      const int unit = first + team;
+      scale_sums(0.0f);
+      for (int band = bands; band >= 0; --band) {
+        cp_wait<0>();
+        __syncthreads();
+        stage_x(band);
+        __syncthreads();
+        start(unit, min(unit + 1, p.units));
+        if (band < bands) scale_sums(0x1p-32f);
+        if (unit < p.units) walk(unit, unit + 1);
+      }
+      if (unit < p.units) finish(unit);
+    }
   }
   cp_wait<0>();
-
-  // The warps' sums, in shared memory [warp][16 MT rows][kCols + 1] over what is no longer needed.
-  constexpr int kPitch = kCols + 1;
-  float* part = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[(warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)] = acc[m][n][e];
-  __syncthreads();
-  const int cols = swiglu ? g.out / 2 : g.out;
-  const int per_tile = swiglu ? 8 : 16;
-  for (int i = threadIdx.x; i < MT * per_tile * g.rows; i += kThreads) {
-    const int r = i / (MT * per_tile), local = i - r * (MT * per_tile), m = local / per_tile, j = local - m * per_tile;
-    const int n = weight_row<NF4>(tile0 + m, j, g.out, swiglu);
-    if (NF4 ? (tile0 + m) * per_tile + j >= cols : n >= cols) continue;
-    float z[2];
-    for (int h = 0; h < (swiglu ? 2 : 1); ++h) {
-      float s = 0.0f;
-      for (int w = 0; w < kWarps; ++w) s += part[(w * MT * 16 + m * 16 + j + 8 * h) * kPitch + r];
-      const int at = n + h * cols;
-      const float b = g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
-      z[h] = ldexpf(s * g.global_scale, row_e[r] - 14) + b;
-    }
-    g.y[size_t(r) * cols + n] = __float2bfloat16(activated(z[0], swiglu ? z[1] : 0.0f, g.act));
-  }
 }
 
 int log2_of(int v) {
@@ -416,41 +451,57 @@ int log2_of(int v) {
 bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-template <bool NF4, int NT, int MT> void launch(const MatvecArgs& g, cudaStream_t stream) {
-  constexpr int D = MT == 1 ? 4 : MT == 2 ? 3 : 2;
+// What a launch with this kernel takes of shared memory for `rows` rows of x.
+template <bool NF4, int NT, int MT, int D> size_t plan(const MatvecArgs& g, int rows, Plan& p) {
   const bool swiglu = g.act == SFQ_ACT_SWIGLU;
   const int tiles = NF4 ? ((swiglu ? g.out / 2 : g.out) + (swiglu ? 7 : 15)) / (swiglu ? 8 : 16) : g.out / 16;
+  p.units = (tiles + MT - 1) / MT;
+  size_t at = NF4 ? kTableBytes : 0;
+  p.ring_off = int(at);
+  at += size_t(kTeams) * kTeamWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
+  p.part_off = int(at);
+  at += size_t(kTeams) * kTeamWarps * MT * 16 * (NT * 8 + 1) * 4;
+  p.x_off = int(at);
+  return at + size_t((g.in + kStep - 1) / kStep * kStep) * rows * 2;
+}
+
+template <bool NF4, int NT, int MT, int D> bool fits(const MatvecArgs& g, int rows) {
   Plan p;
-  int at = NF4 ? kTableBytes : 0;
-  p.absmax_off = at;
-  if (NF4) p.groups = g.in / 64, at += (MT * 16 * p.groups + 15) / 16 * 16;
-  p.x_off = at;
-  constexpr int kTurn = kWarps * kStep;
-  const int whole = (g.in + kTurn - 1) / kTurn * kTurn;
-  p.slab = std::max(kTurn, std::min(whole, 81920 / (2 * g.rows) / kTurn * kTurn));
-  at += std::min(p.slab, (g.in + kStep - 1) / kStep * kStep) * g.rows * 2;
-  p.ring_off = at;
-  at += kWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
-  at = std::max(at, kWarps * MT * 16 * (NT * 8 + 1) * 4);
-  if (at > 230000) throw std::invalid_argument("matvec: in_features too large");
-  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT>), size_t(at), "matvec");
-  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT>, dim3((tiles + MT - 1) / MT), dim3(kThreads), size_t(at), stream, g, p);
+  return plan<NF4, NT, MT, D>(g, rows, p) <= kMostSmem;
+}
+
+template <bool NF4, int NT, int MT, int D> void launch(const MatvecArgs& g, cudaStream_t stream) {
+  Plan p;
+  const size_t bytes = plan<NF4, NT, MT, D>(g, g.rows, p);
+  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT, D>), bytes, "matvec");
+  const int resident = !NF4 && D == 4 && bytes <= kMostSmem / 2 - 1024 ? 2 : 1;
+  const int ctas = std::min((p.units + kTeams - 1) / kTeams, resident * device_sm_count());
+  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT, D>, dim3(ctas), dim3(kThreads), bytes, stream, g, p);
   if (e != cudaSuccess) throw std::runtime_error(std::string("matvec: launch failed: ") + cudaGetErrorString(e));
 }
 
-template <bool NF4> void launch_rows(const MatvecArgs& g, cudaStream_t stream) {
-  const int tiles = NF4 ? (g.out + 15) / 16 : g.out / 16;
-  int mt = g.rows <= 2 ? 1 : g.rows <= 4 ? 2 : 4;
-  while (mt > 1 && tiles < mt * device_sm_count()) mt /= 2;
-  while (NF4 && mt > 1 && mt * g.in > 131072) mt /= 2;  // the absmax bytes of the tiles' rows
-  if (g.rows <= 8) {
-    if (mt == 1) launch<NF4, 1, 1>(g, stream);
-    else if (mt == 2) launch<NF4, 1, 2>(g, stream);
-    else launch<NF4, 1, 4>(g, stream);
-  } else {
-    if (mt == 1) launch<NF4, 2, 1>(g, stream);
-    else if (mt == 2) launch<NF4, 2, 2>(g, stream);
-    else launch<NF4, 2, 4>(g, stream);
+template <bool NF4> void launch_rows(MatvecArgs g, int cols, cudaStream_t stream) {
+  if (!fits<NF4, 1, 1, 2>(g, 1)) throw std::invalid_argument("matvec: in_features too large");
+  int rows = g.rows;
+  while (rows > 0) {
+    // as many rows at a time as x fits into shared memory for, in equal parts
+    int most = std::min(rows, kMostRows);
+    while (most > 1 && !(most > 8 ? fits<NF4, 2, 1, 2>(g, most) : fits<NF4, 1, 1, 2>(g, most))) --most;
+    const int parts = (rows + most - 1) / most;
+    g.rows = (rows + parts - 1) / parts;
+    if (g.rows > 8)
+      launch<NF4, 2, 1, 2>(g, stream);
+    else if (g.rows <= 2 && fits<NF4, 1, 1, 4>(g, g.rows))
+      launch<NF4, 1, 1, 4>(g, stream);
+    else if (fits<NF4, 1, 2, 3>(g, g.rows) && g.out >= 32 * kTeams * device_sm_count())
+      launch<NF4, 1, 2, 3>(g, stream);
+    else if (fits<NF4, 1, 1, 4>(g, g.rows))
+      launch<NF4, 1, 1, 4>(g, stream);
+    else
+      launch<NF4, 1, 1, 2>(g, stream);
+    rows -= g.rows;
+    g.x += size_t(g.rows) * g.in;
+    g.y += size_t(g.rows) * cols;
   }
 }
 
@@ -478,17 +529,10 @@ void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream
     const auto x0 = reinterpret_cast<uintptr_t>(g.x), x1 = x0 + size_t(g.rows) * g.in * 2, y0 = reinterpret_cast<uintptr_t>(g.y), y1 = y0 + size_t(g.rows) * cols * 2;
     if (x0 < y1 && y0 < x1) throw std::invalid_argument("matvec: x and y may not overlap");
   }
-  const int rows = g.rows;
-  for (int r = 0; r < rows; r += kMostRows) {
-    MatvecArgs part = g;
-    part.rows = std::min(rows - r, kMostRows);
-    part.x = g.x + size_t(r) * g.in;
-    part.y = g.y + size_t(r) * cols;
-    if (g.nf4)
-      launch_rows<true>(part, stream);
-    else
-      launch_rows<false>(part, stream);
-  }
+  if (g.nf4)
+    launch_rows<true>(g, cols, stream);
+  else
+    launch_rows<false>(g, cols, stream);
 }
 
 }  // namespace sfq
