@@ -42,10 +42,16 @@ struct Plan {
 };
 
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
+__device__ __forceinline__ void cp_async4_or_zero(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -140,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
   const int steps = (g.in + kStep - 1) / kStep;
   const uint32_t base = smem_u32(smem);
   const uint32_t ring = base + p.ring_off + (threadIdx.x >> 5) * D * kStage;
-  const int first_unit = blockIdx.x * kTeams + team, all_teams = gridDim.x * kTeams;
+  const int first_unit = team * gridDim.x + blockIdx.x, all_teams = gridDim.x * kTeams;  // what is left over falls on different CTAs
   grid_dependency_release();
 
   // The copies under way: the next one is step `fs` of unit `fu`.
@@ -159,24 +165,28 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
         scale_src[m] = g.scale + nvfp4_scale_offset(weight_row<NF4>(unit * MT + m, lane & 15, g.out, swiglu), (lane >> 4) * 4, g.in / 16) + size_t(warp) * (kStep * 8);
     }
   };
-  auto fetch = [&](int slot, int end_unit) {  // elements past the end of a row are zeros
+  const uint32_t code_at = gq * 64 + (NF4 ? q ^ (gq & 2) : q) * 16;  // in a tile's codes; NF4 is read in 8-byte pieces of four rows at a time
+  auto fetch = [&](uint32_t to, int end_unit) {
     if (fs < steps && fu < end_unit) {
-      const uint32_t to = ring + slot * kStage;
-      const bool live = fs * kStep + q * 32 < g.in;
+      if ((fs + 1) * kStep <= g.in) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          cp_async16(to + m * 1024 + code_at, src[m][0]);
+          cp_async16(to + m * 1024 + code_at + 512, src[m][1]);
+          if constexpr (!NF4) cp_async4(to + MT * 1024 + m * 128 + lane * 4, scale_src[m]);
+        }
+      } else {  // the half step at the end of a row: zeros in the place of the rest
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          cp_async16_or_zero(to + m * 1024 + code_at, q < 2 ? src[m][0] : g.data, q < 2);
+          cp_async16_or_zero(to + m * 1024 + code_at + 512, q < 2 ? src[m][1] : g.data, q < 2);
+          if constexpr (!NF4) cp_async4_or_zero(to + MT * 1024 + m * 128 + lane * 4, lane < 16 ? scale_src[m] : g.scale, lane < 16);
+        }
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = gq + 8 * h;
-          const int unit = NF4 ? q ^ (row & 2) : q;  // NF4 is read in 8-byte pieces of four rows at a time
-          cp_async16(to + m * 1024 + row * 64 + unit * 16, live ? src[m][h] : g.data, live);
-          src[m][h] += kTeamWarps * kStep / 2;
-        }
-        if constexpr (!NF4) {
-          const bool there = fs * kStep + (lane >> 4) * 64 < g.in;
-          cp_async4(to + MT * 1024 + m * 128 + lane * 4, there ? scale_src[m] : g.scale, there);
-          scale_src[m] += kTeamWarps * kStep * 8;
-        }
+        src[m][0] += kTeamWarps * kStep / 2, src[m][1] += kTeamWarps * kStep / 2;
+        if constexpr (!NF4) scale_src[m] += kTeamWarps * kStep * 8;
       }
       fs += kTeamWarps;
       if (fs >= steps) seek(fu + all_teams);
@@ -184,14 +194,21 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
     cp_commit();
   };
   // NF4: lane l holds the absmax of row l / 2, group l % 2 of a step: its byte and its nested scale, fetched a step ahead.
+  const int last_group = g.in / 64 - 1;
   uint32_t absmax_byte[MT];
-  float absmax_outer[MT];
-  auto fetch_absmax = [&](int unit, int s) {
+  float absmax_outer[MT], absmax[MT];
+  size_t absmax_row[MT];  // its row's first element
+  auto seek_absmax = [&](int unit) {
+    if constexpr (NF4) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) absmax_row[m] = size_t(weight_row<true>(unit * MT + m, lane >> 1, g.out, swiglu)) * g.in;
+    }
+  };
+  auto fetch_absmax = [&](int s) {
     if constexpr (NF4) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const int group = min(s * 2 + (lane & 1), g.in / 64 - 1);
-        const size_t block = (size_t(weight_row<true>(unit * MT + m, lane >> 1, g.out, swiglu)) * g.in + size_t(group) * 64) >> g.block_shift;
+        const size_t block = (absmax_row[m] + uint32_t(min(s * 2 + (lane & 1), last_group)) * 64) >> g.block_shift;
         absmax_byte[m] = g.scale[block], absmax_outer[m] = g.nested_absmax[block >> g.nested_shift];
       }
     }
@@ -243,9 +260,13 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
     if (band < 0 && (low != 0 || fmaxf(__low2float(top), __high2float(top)) >= 1024.0f)) flags = 1;
   };
 
-  auto multiply = [&](int s, int slot) {
-    const uint32_t from = ring + slot * kStage;
-    const uint32_t xs = base + p.x_off + (s * 4 * g.rows * 4 + lane) * 16;
+  // Lanes of columns that stand for no row of x read another row's; what they add up is not stored.
+  uint32_t x_at[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) x_at[n] = base + p.x_off + (min(gq + 8 * n, g.rows - 1) * 4 + q) * 16;
+  const uint32_t x_piece = g.rows * 64;
+  auto multiply = [&](int s, uint32_t from) {
+    const uint32_t xs = s * 4 * x_piece;
     if constexpr (!NF4) {
       uint4 w[MT][2];
       uint32_t sc[MT][2];
@@ -261,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
       for (int j = 0; j < 4; ++j) {
         uint4 xv[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) xv[n] = gq + 8 * n < g.rows ? lds128(xs + (j * g.rows + 8 * n) * 64) : make_uint4(0, 0, 0, 0);
+        for (int n = 0; n < NT; ++n) xv[n] = lds128(x_at[n] + xs + j * x_piece);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           uint32_t a[2][4];
@@ -279,17 +300,14 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
       }
     } else {
       const uint32_t lane4 = lane * 4;
-      float absmax[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) absmax[m] = fmaf(nested_map[absmax_byte[m]], absmax_outer[m], g.offset);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if (s * 2 + c >= g.in / 64) break;
+        if (s * 2 + c > last_group) break;
         uint4 xv[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) xv[n][j] = gq + 8 * n < g.rows ? lds128(xs + ((c * 2 + j) * g.rows + 8 * n) * 64) : make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 2; ++j) xv[n][j] = lds128(x_at[n] + xs + (c * 2 + j) * x_piece);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           uint2 w[2];
@@ -329,26 +347,35 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
   };
 
   // This warp's steps of a unit. Their first D - 1 copies are under way, and go on with the units up to end_unit.
-  int slot = 0;
+  uint32_t slot = 0;  // byte offset into the ring
   auto walk = [&](int unit, int end_unit) {
     for (int s = warp; s < steps; s += kTeamWarps) {
-      fetch(slot == 0 ? D - 1 : slot - 1, end_unit);
-      cp_wait<D - 1>();
-      __syncwarp();
-      multiply(s, slot);
-      if (s + kTeamWarps < steps)
-        fetch_absmax(unit, s + kTeamWarps);
-      else if (unit + all_teams < end_unit)
-        fetch_absmax(unit + all_teams, warp);
-      __syncwarp();
-      slot = slot == D - 1 ? 0 : slot + 1;
+      cp_wait<D - 2>();
+      __syncwarp();  // the copies have landed in every lane, and the step in front has been read
+      fetch(ring + (slot == 0 ? (D - 1) * kStage : slot - kStage), end_unit);
+      if constexpr (NF4) {  // this step's absmax, and the loads of the next one's, which have the products' time to arrive
+#pragma unroll
+        for (int m = 0; m < MT; ++m) absmax[m] = fmaf(nested_map[absmax_byte[m]], absmax_outer[m], g.offset);
+        if (s + kTeamWarps < steps) {
+          fetch_absmax(s + kTeamWarps);
+        } else if (unit + all_teams < end_unit) {
+          seek_absmax(unit + all_teams);
+          fetch_absmax(warp);
+        }
+      }
+      multiply(s, ring + slot);
+      slot = slot == (D - 1) * kStage ? 0 : slot + kStage;
     }
   };
   auto start = [&](int unit, int end_unit) {
     slot = 0;
+    __syncwarp();
     seek(unit);
-    for (int i = 0; i < D - 1; ++i) fetch(i, end_unit);
-    if (unit < end_unit && warp < steps) fetch_absmax(unit, warp);
+    for (int i = 0; i < D - 1; ++i) fetch(ring + i * kStage, end_unit);
+    if (unit < end_unit && warp < steps) {
+      seek_absmax(unit);
+      fetch_absmax(warp);
+    }
   };
 
   // The team's sums of a unit, added in the order of its warps, finished and stored.
@@ -425,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
       finish(unit);
     }
   } else {
-    for (int first = blockIdx.x * kTeams; first < p.units; first += all_teams) {  // the teams in step, since x changes under them
-      const int unit = first + team;
+    for (int first = blockIdx.x; first < p.units; first += all_teams) {  // the teams in step, since x changes under them
+      const int unit = first + team * gridDim.x;
       scale_sums(0.0f);
       for (int band = bands; band >= 0; --band) {
         cp_wait<0>();
