@@ -144,7 +144,7 @@ def _load() -> C.CDLL:
         "sfq_attention_forward": (I, [V, I, V, V, I, V, I, I, I, I, I, I, C.c_float, V, SZ, V]),
         "sfq_linear_matvec": (I, [P(QuantWeight), V, I, I, V, V]),
         "sfq_kv_cache_append": (I, [P(KvCacheDesc), P(RotaryDesc), V, I, V, I, I, V, V, I, I, V]),
-        "sfq_kv_cache_attention_workspace_bytes": (I, [P(KvCacheDesc), I, P(SZ)]),
+        "sfq_kv_cache_attention_workspace_bytes": (I, [P(KvCacheDesc), I, I, P(SZ)]),
         "sfq_kv_cache_attention": (I, [P(KvCacheDesc), V, I, V, I, I, I, C.c_float, V, SZ, V]),
         "sfq_lora_create": (I, [P(V)]),
         "sfq_lora_destroy": (None, [V]),

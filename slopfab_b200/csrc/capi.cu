@@ -431,11 +431,11 @@ int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rotary, con
     sfq::kv_append(v, cache->head_dim, r, a, as_stream(stream));
   });
 }
-int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, size_t* out) {
+int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, int rows, size_t* out) {
   return guarded([&] {
     if (!out) throw std::invalid_argument("sfq_kv_cache_attention_workspace_bytes: null output");
-    const sfq::KvCacheView v = to_cache(cache, 0);
-    *out = sfq::kv_attention_workspace_bytes(v, cache->head_dim, heads);
+    const sfq::KvCacheView v = to_cache(cache, rows);
+    *out = sfq::kv_attention_workspace_bytes(v, cache->head_dim, heads, rows);
   });
 }
 int sfq_kv_cache_attention(const sfq_kv_cache* cache, const void* d_q_bf16, int ld_q, void* d_out_bf16, int ld_out, int heads, int rows, float scale,

@@ -141,7 +141,7 @@ struct KvAttentionArgs {
 };
 void kv_check(const KvCacheView& c, int head_dim);
 void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendArgs& g, cudaStream_t stream);
-size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads);
+size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads, int rows);
 void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 // LoRA side branch in one launch (lora_kernel.cu): y[rows,out] += bf16(bf16(x a^T) b^T), a [rank,in], b [out,rank]; false,

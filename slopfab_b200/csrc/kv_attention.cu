@@ -1,13 +1,22 @@
 // Attention of a few new tokens per sequence over the paged 8-bit cache, grouped heads, causal among the new tokens.
 //
-// Bound by memory: every sequence's e4m3 codes of K and V are read once, 256 bytes for a token and kv head.
-#include <cuda_fp8.h>
+// Bound by memory: every sequence's e4m3 codes of K and V are read once, 256 bytes for a token and kv head, and each is one conversion of
+// half an instruction away from fp16. The products run on mma.sync m16n8k16, transposed, so that the query heads of a group (and the new
+// tokens of a sequence), of which there are few, are its N of 8 and the cache its M of 16:
+//   S^T [tokens, queries] = K Q^T    O^T [channels, queries] += V^T P^T
+// A warp takes 64 tokens at a time. V lies with a channel's tokens side by side, so both operands are 16-byte loads straight into
+// registers, and the weights P go from the first product's result to the second one's operand by 8 x 8 transposes between lanes. Which
+// token is which row of the first product is free: the order is chosen so that the transposed weights of four MMAs meet the 16
+// neighbouring tokens of a lane's V. Softmax with running maximum and sum in fp32; the page's scale of K goes into the score, that of V into
+// the weight.
+// Long sequences are divided over CTAs (flash decoding); a second launch joins their parts in order.
+#include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <stdexcept>
 #include <string>
 
-#include "codec.cuh"
 #include "kv_cache.cuh"
 #include "ptx.cuh"
 #include "runtime.h"
@@ -17,73 +26,510 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 64;        // tokens a warp takes at a time
+constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
+constexpr int kMostSplits = 64;
 
-// One warp per (row, head): a lane holds four channels, one key after the other with the running maximum and sum.
-__global__ void __launch_bounds__(kWarps * 32) kv_attention_kernel(KvCacheView c, KvAttentionArgs g) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four e4m3 of a word as two pairs of fp16.
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint4 load_cache(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// 0xFF in the bytes of w that are NaN (0x7F or 0xFF).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
+  constexpr int kCols = NT * 8;
+  __shared__ float sh_o[kWarps][128 * (kCols + 1)];
+  __shared__ float sh_m[kWarps][kCols], sh_mv[kWarps][kCols], sh_l[kWarps][kCols];
+  __shared__ int sh_seen[kWarps][kCols];
+  __shared__ uint2 sh_q[8][NT][32];
+  __shared__ float sh_qscale[kCols];
+  grid_dependency_release();
+  grid_dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
+  const int head = blockIdx.y, split = int(blockIdx.x) % splits;
+  const int page_mask = (1 << c.page_shift) - 1;
+
+  for (int b = blockIdx.z; b < c.batch; b += gridDim.z) {
+    const KvSequence s = kv_sequence(c, b);
+    // Lengths are 32-bit; the last few thousand of their range are not used, so that sums of places stay in it.
+    const int length = int(max(0ll, min(min(s.length, (long long)c.max_pages << c.page_shift), 0x7FFF0000ll)));
+    const int past = int(max(-0x7FFF0000ll, min(s.length, 0x7FFF0000ll) - s.rows));  // tokens in front of the new ones
+    const int all_cols = s.rows * g.group;
+    for (int col0 = int(blockIdx.x) / splits * kCols; col0 < all_cols; col0 += int(gridDim.x) / splits * kCols) {
+      __syncthreads();  // what the tile in front left in shared memory has been read
+      // ---- the queries as fp16, each times a power of two that takes its largest element just below 2^15. Its eight significant bits are
+      // exact down to 2^-31 of that; what is smaller is off by 2^-39 of it at most.
+      for (int i = threadIdx.x; i < kCols * 4; i += kThreads) {
+        const int col = i >> 2, quarter = i & 3;
+        const int at = min(col0 + col, all_cols - 1), token = at / g.group, qh = head * g.group + at % g.group;
+        const __nv_bfloat16* src = g.q + size_t(s.row0 + token) * g.ld_q + qh * kKvHeadDim + quarter * 16;
+        uint32_t raw[16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src + (u >> 1) * 64 + (u & 1) * 8);
+          raw[4 * u] = v.x, raw[4 * u + 1] = v.y, raw[4 * u + 2] = v.z, raw[4 * u + 3] = v.w;
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const uint32_t lo = raw[u] & 0x7FFFu, hi = (raw[u] >> 16) & 0x7FFFu;
+          if (lo < 0x7F80u) top = max(top, lo);
+          if (hi < 0x7F80u) top = max(top, hi);
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(int(top >> 7), 1) - 127;  // exponent of the largest element
+        const float up = ldexpf(1.0f, min(14 - e, 127)), up2 = ldexpf(1.0f, 14 - e - min(14 - e, 127));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t r = raw[2 * j + h];
+            w[h] = half_pair(__uint_as_float(r << 16) * up * up2, __uint_as_float(r & 0xFFFF0000u) * up * up2);
+          }
+          sh_q[j][col >> 3][(col & 7) * 4 + quarter] = make_uint2(w[0], w[1]);
+        }
+        if (quarter == 0) sh_qscale[col] = ldexpf(g.scale_log2, e - 14);
+      }
+      __syncthreads();
+
+      // ---- this warp's columns, state and tokens
+      int sees[NT][2];
+      float qscale[NT][2], m[NT][2], mv[NT][2], l[NT][2];
+      bool seen[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = n * 8 + q * 2 + e;
+          sees[n][e] = min(length, past + min(col0 + col, all_cols - 1) / g.group + 1);
+          qscale[n][e] = sh_qscale[col];
+          m[n][e] = mv[n][e] = -INFINITY, l[n][e] = 0.0f, seen[n][e] = false;
+        }
+      const int last = min(length, past + min(col0 + kCols - 1, all_cols - 1) / g.group + 1);  // keys that any column sees
+      const int first_hidden = past + col0 / g.group + 1;  // ... that one of them does not
+      const int tiles = (max(last, 0) + kTile - 1) / kTile, per_split = (tiles + splits - 1) / splits;
+      const int tile_end = min(tiles, (split + 1) * per_split);
+      float o[8][NT][4];
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.0f;
+
+      // K is read by the lane whose rows lie in chunk gq / 2 of the tile's four chunks of 16 tokens, V in chunk q.
+      auto page_of = [&](int tile, int chunk) -> int {
+        const int t = tile * kTile + chunk * 16;
+        return tile < tile_end && t < last ? kv_page(c, b, t >> c.page_shift) : -1;
+      };
+      // One query tile has the registers for a tile's K under the products of the one in front.
+      constexpr bool kAhead = NT == 1;
+      uint4 kraw[kAhead ? 4 : 1][4];
+      const uint8_t* k_at = c.k;
+      int k_step = 0;
+      auto seek_k = [&](int tile, int page) {
+        const int slot = (tile * kTile + (gq >> 1) * 16) & page_mask;
+        k_at = page < 0 ? c.k : c.k + (((size_t(page) * c.kv_heads + head) << c.page_shift) + slot + (gq & 1)) * kKvHeadDim + q * 16;
+        k_step = page < 0 ? 0 : 1;  // a chunk that is not there: any bytes
+      };
+      auto load_k = [&](int t, uint4 (&to)[4]) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) to[u] = load_cache(k_at + k_step * ((t * 4 + (u >> 1) * 2) * kKvHeadDim + (u & 1) * 64));
+      };
+      auto load_ahead = [&](int tile, int page) {
+        seek_k(tile, page);
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) load_k(t, kraw[t]);
+        }
+      };
+      int tile = split * per_split + warp;
+      int page_k = page_of(tile, gq >> 1), page_v = page_of(tile, q);
+      int next_k = page_of(tile + kWarps, gq >> 1), next_v = page_of(tile + kWarps, q);
+      if (tile < tile_end) load_ahead(tile, page_k);
+      for (; tile < tile_end; tile += kWarps) {
+        const int t0 = tile * kTile;
+        // ---- V of this tile on its way
+        uint4 vraw[8][2];
+        auto load_v = [&] {
+          const int slot = (tile * kTile + q * 16) & page_mask;
+          const uint8_t* p = page_v < 0 ? c.v : c.v + (((size_t(page_v) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
+          const int step = page_v < 0 ? 0 : 8 << c.page_shift;
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vraw[d][h] = load_cache(p + (d * 2 + h) * step);
+        };
+        if constexpr (kAhead) load_v();
+        const float ks = page_k < 0 ? 0.0f : c.k_scale[size_t(page_k) * c.kv_heads + head];
+        const float vs = page_k < 0 ? 0.0f : c.v_scale[size_t(page_k) * c.kv_heads + head];
+        // ---- scores
+        float sc[4][NT][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sc[t][n][0] = sc[t][n][1] = sc[t][n][2] = sc[t][n][3] = 0.0f;
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint2 bq[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) bq[n] = sh_q[j][n][lane];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              uint32_t a0, a1, a2, a3;
+              e4m3_pairs(word_of(kraw[t][j >> 2], j & 3), a0, a2);
+              e4m3_pairs(word_of(kraw[t][2 + (j >> 2)], j & 3), a1, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(sc[t][n], a0, a1, a2, a3, bq[n].x, bq[n].y);
+            }
+          }
+        } else {
+          uint4 two[2][4];
+          load_k(0, two[0]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if (t < 3) load_k(t + 1, two[(t + 1) & 1]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t a0, a1, a2, a3;
+              e4m3_pairs(word_of(two[t & 1][j >> 2], j & 3), a0, a2);
+              e4m3_pairs(word_of(two[t & 1][2 + (j >> 2)], j & 3), a1, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                const uint2 bq = sh_q[j][n][lane];
+                mma_f16(sc[t][n], a0, a1, a2, a3, bq.x, bq.y);
+              }
+            }
+          }
+          load_v();
+        }
+        const int page = page_k;
+        page_k = next_k;
+        if (tile + kWarps < tile_end) load_ahead(tile + kWarps, page_k);
+        // ---- weights
+        const bool whole = __all_sync(0xffffffffu, page >= 0) && t0 + kTile <= min(first_hidden, length);
+        const int mine = t0 + (gq >> 1) * 16 + (gq & 1);  // token of row gq of MMA 0; row gq + 8 is two behind, MMA t four t
+        // The weights of the second product are p vs = exp2(score + e) (vs / 2^e) with vs / 2^e in [0.5, 1), over their own running
+        // reference mv, the largest score + e: a page of small values that has all the weight keeps its bits beside one of large values
+        // that has none.
+        const float e_mine = vs > 0.0f ? float(min(ilogbf(vs), 127) + 1) : 0.0f;
+        const float frac = vs > 0.0f ? ldexpf(vs, -int(e_mine)) : vs;
+        float top[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float v = sc[t][n][e] * (ks * qscale[n][e & 1]);
+              if (!whole) {
+                const bool there = page >= 0 && mine + t * 4 + (e >> 1) * 2 < sees[n][e & 1];
+                seen[n][e & 1] |= there;
+                v = there ? v : -INFINITY;
+              }
+              sc[t][n][e] = v;
+              top[n][e & 1] = fmaxf(top[n][e & 1], v);
+            }
+          if (whole) seen[n][0] = seen[n][1] = true;
+        }
+        float top_v[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) top_v[n][0] = top[n][0] + e_mine, top_v[n][1] = top[n][1] + e_mine;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], off));
+              top_v[n][e] = fmaxf(top_v[n][e], __shfl_xor_sync(0xffffffffu, top_v[n][e], off));
+            }
+        float keep[NT][2];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float m_new = fmaxf(m[n][e], top[n][e]), mv_new = fmaxf(mv[n][e], top_v[n][e]);
+            l[n][e] *= m_new == -INFINITY ? 1.0f : exp2f(m[n][e] - m_new);  // exp2(-inf - x) = 0 on the first tile
+            keep[n][e] = mv_new == -INFINITY ? 1.0f : exp2f(mv[n][e] - mv_new);
+            moved |= mv_new != mv[n][e];
+            m[n][e] = m_new, mv[n][e] = mv_new;
+          }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][n][e] *= keep[n][e & 1];
+        }
+        uint32_t p[4][NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float ref[2], ref_v[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            ref[e] = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+            ref_v[e] = e_mine - (mv[n][e] == -INFINITY ? 0.0f : mv[n][e]);
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              l[n][e & 1] += exp2f(sc[t][n][e] - ref[e & 1]);
+              w[e] = exp2f(sc[t][n][e] + ref_v[e & 1]) * frac;
+            }
+            p[t][n][0] = transpose8x8(half_pair(w[0], w[1]));
+            p[t][n][1] = transpose8x8(half_pair(w[2], w[3]));
+          }
+        }
+        // ---- V behind the sequence's end, or of no page, is zeros: a weight of zero does not undo NaN bytes
+        const int v0 = t0 + q * 16;
+        if (t0 + kTile > length || !__all_sync(0xffffffffu, page_v >= 0)) {
+          const int live = page_v < 0 ? 0 : max(0, min(16, length - v0));
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int bytes = min(max(live - 4 * w, 0), 4);
+            const uint32_t mask = bytes == 4 ? 0xFFFFFFFFu : (1u << (8 * bytes)) - 1u;
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) (w == 0 ? vraw[d][h].x : w == 1 ? vraw[d][h].y : w == 2 ? vraw[d][h].z : vraw[d][h].w) &= mask;
+          }
+        }
+        if (t0 + kTile > first_hidden) {
+          // Tokens that some of the columns do not see: NaN among their values may reach only those that do. They are taken out of V, and
+          // a product of their places with who sees what says where they belong.
+          uint32_t any = 0;
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) any |= nan_bytes(word_of(vraw[d][h], w));
+          if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll 1
+            for (int n = 0; n < NT; ++n) {
+              const int sees_mine = min(length, past + min(col0 + n * 8 + gq, all_cols - 1) / g.group + 1);
+#pragma unroll
+              for (int d = 0; d < 8; ++d) {
+                float places[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                  uint32_t a[2][2], bsee[2];
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const uint32_t bad = nan_bytes(word_of(vraw[d][h], t)) & 0x38383838u;  // e4m3 1.0
+                    e4m3_pairs(bad, a[h][0], a[h][1]);
+                  }
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int at = v0 + t * 4 + h * 2;
+                    bsee[h] = (at < sees_mine ? 0x3C00u : 0u) | (at + 1 < sees_mine ? 0x3C000000u : 0u);
+                  }
+                  mma_f16(places, a[0][0], a[1][0], a[0][1], a[1][1], bsee[0], bsee[1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                  for (int k = 0; k < NT; ++k)
+                    if (k == n && places[e] != 0.0f) o[d][k][e] = NAN;
+              }
+            }
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                vraw[d][h].x &= ~nan_bytes(vraw[d][h].x), vraw[d][h].y &= ~nan_bytes(vraw[d][h].y);
+                vraw[d][h].z &= ~nan_bytes(vraw[d][h].z), vraw[d][h].w &= ~nan_bytes(vraw[d][h].w);
+              }
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            uint32_t a0, a1, a2, a3;
+            e4m3_pairs(word_of(vraw[d][0], t), a0, a2);
+            e4m3_pairs(word_of(vraw[d][1], t), a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(o[d][n], a0, a1, a2, a3, p[t][n][0], p[t][n][1]);
+          }
+        page_v = next_v;
+        next_k = page_of(tile + 2 * kWarps, gq >> 1), next_v = page_of(tile + 2 * kWarps, q);
+      }
+
+      // ---- the four warps joined
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
+            seen[n][e] |= __shfl_xor_sync(0xffffffffu, int(seen[n][e]), off) != 0;
+          }
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sh_o[warp][(d * 16 + gq + (e >> 1) * 8) * (kCols + 1) + n * 8 + q * 2 + (e & 1)] = o[d][n][e];
+      if (gq == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = n * 8 + q * 2 + e;
+            sh_m[warp][col] = m[n][e], sh_mv[warp][col] = mv[n][e], sh_l[warp][col] = l[n][e], sh_seen[warp][col] = seen[n][e];
+          }
+      }
+      __syncthreads();
+      const int cols = min(kCols, all_cols - col0);
+      for (int i = threadIdx.x; i < cols * 32; i += kThreads) {
+        const int col = i >> 5, d4 = (i & 31) * 4;
+        float mm = -INFINITY, ll = 0.0f, sum[4] = {0, 0, 0, 0};
+        bool any = false;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sh_m[w][col]), any |= sh_seen[w][col] != 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (sh_seen[w][col] == 0) continue;
+          const float ref = mm == -INFINITY ? 0.0f : mm;
+          ll = fmaf(sh_l[w][col], sh_m[w][col] == -INFINITY && sh_l[w][col] == 0.0f ? 0.0f : exp2f(sh_m[w][col] - ref), ll);
+          const float f = sh_mv[w][col] == -INFINITY ? 1.0f : exp2f(sh_mv[w][col] - ref);  // a part without a finite score is 0 or NaN
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[k] = fmaf(sh_o[w][(d4 + k) * (kCols + 1) + col], f, sum[k]);
+        }
+        const int at = col0 + col, row = s.row0 + at / g.group, qh = head * g.group + at % g.group;
+        if (splits > 1) {
+          float* part = parts + ((size_t(row) * g.heads + qh) * splits + split) * kPartFloats;
+          *reinterpret_cast<float4*>(part + d4) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+          if (d4 == 0) *reinterpret_cast<float4*>(part + 128) = make_float4(mm, ll, any ? 1.0f : 0.0f, 0.0f);
+        } else {
+          const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;  // keys but no finite score: NaN; no key: zeros
+          uint2 v;
+          __nv_bfloat162 lo = __floats2bfloat162_rn(sum[0] * inv, sum[1] * inv), hi = __floats2bfloat162_rn(sum[2] * inv, sum[3] * inv);
+          v.x = *reinterpret_cast<const uint32_t*>(&lo), v.y = *reinterpret_cast<const uint32_t*>(&hi);
+          *reinterpret_cast<uint2*>(g.out + size_t(row) * g.ld_out + qh * kKvHeadDim + d4) = v;
+        }
+      }
+    }
+  }
+}
+
+// One warp per row and head: its parts in order.
+__global__ void __launch_bounds__(kThreads) kv_join_kernel(KvCacheView c, KvAttentionArgs g, const float* parts, int splits) {
   grid_dependency_release();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  const int page_size = 1 << c.page_shift;
   for (int b = blockIdx.y; b < c.batch; b += gridDim.y) {
     const KvSequence s = kv_sequence(c, b);
-    for (long long unit = blockIdx.x * kWarps + int(threadIdx.x >> 5); unit < (long long)s.rows * g.heads; unit += gridDim.x * kWarps) {
-      const int i = int(unit / g.heads), head = int(unit % g.heads), kv_head = head / g.group;
-      const __nv_bfloat16* q = g.q + size_t(s.row0 + i) * g.ld_q + head * kKvHeadDim + lane * 4;
-      float qv[4], o[4] = {0, 0, 0, 0}, m = -FLT_MAX, sum = 0.0f;
-      for (int e = 0; e < 4; ++e) qv[e] = __bfloat162float(q[e]);
+    for (long long unit = (long long)blockIdx.x * kWarps + int(threadIdx.x >> 5); unit < (long long)s.rows * g.heads; unit += gridDim.x * kWarps) {
+      const int row = s.row0 + int(unit / g.heads), qh = int(unit % g.heads);
+      const float* part = parts + (size_t(row) * g.heads + qh) * splits * kPartFloats;
+      float mm = -INFINITY, ll = 0.0f, sum[4] = {0, 0, 0, 0};
       bool any = false;
-      const long long sees = min(s.length - s.rows + i + 1, (long long)c.max_pages << c.page_shift);
-      for (long long t = 0; t < sees; ++t) {
-        const int page = kv_page(c, b, t >> c.page_shift);
-        if (page < 0) continue;
+      for (int i = 0; i < splits; ++i) mm = fmaxf(mm, part[i * kPartFloats + 128]);
+      for (int i = 0; i < splits; ++i) {
+        const float4 st = *reinterpret_cast<const float4*>(part + i * kPartFloats + 128), o = *reinterpret_cast<const float4*>(part + i * kPartFloats + lane * 4);
+        if (st.z == 0.0f) continue;
         any = true;
-        const size_t block = size_t(page) * c.kv_heads + kv_head;
-        const int slot = int(t & (page_size - 1));
-        const uint8_t* k = c.k + (block * page_size + slot) * kKvHeadDim + lane * 4;
-        float score = 0.0f;
-        for (int e = 0; e < 4; ++e) score = fmaf(qv[e], e4m3_decode(k[e]), score);
-        for (int off = 16; off > 0; off >>= 1) score += __shfl_xor_sync(0xffffffffu, score, off);
-        score *= c.k_scale[block] * g.scale_log2;
-        float m_new = score > m ? score : m;
-        if (!(score < INFINITY)) m_new = NAN;  // a NaN or +inf score makes its row NaN
-        if (m != m) m_new = m;
-        const float p = exp2f(score - m_new), keep = exp2f(m - m_new);
-        m = m_new;
-        sum = fmaf(sum, keep, p);
-        const float pv = p * c.v_scale[block];
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], keep, pv * e4m3_decode(c.v[(block * kKvHeadDim + lane * 4 + e) * page_size + slot]));
+        const float f = st.x == -INFINITY && st.y == 0.0f ? 0.0f : exp2f(st.x - (mm == -INFINITY ? 0.0f : mm));
+        ll = fmaf(st.y, f, ll);
+        sum[0] = fmaf(o.x, f, sum[0]), sum[1] = fmaf(o.y, f, sum[1]), sum[2] = fmaf(o.z, f, sum[2]), sum[3] = fmaf(o.w, f, sum[3]);
       }
-      const float inv = any ? (m > -FLT_MAX ? 1.0f / sum : NAN) : 0.0f;  // no key: zeros; no finite score: NaN
-      __nv_bfloat16* out = g.out + size_t(s.row0 + i) * g.ld_out + head * kKvHeadDim + lane * 4;
-      for (int e = 0; e < 4; ++e) out[e] = __float2bfloat16(o[e] * inv);
+      const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;
+      __nv_bfloat162 lo = __floats2bfloat162_rn(sum[0] * inv, sum[1] * inv), hi = __floats2bfloat162_rn(sum[2] * inv, sum[3] * inv);
+      *reinterpret_cast<uint2*>(g.out + size_t(row) * g.ld_out + qh * kKvHeadDim + lane * 4) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
   }
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+struct AttentionPlan {
+  int nt, col_tiles, splits;
+};
+
+// How a launch is divided, from the host's estimates.
+AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
+  AttentionPlan p;
+  const long long cols = (long long)std::min(c.max_new, rows) * (heads / c.kv_heads);
+  p.nt = cols > 8 ? 2 : 1;
+  p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
+  const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
+  const long long want = (4ll * device_sm_count() + ctas - 1) / ctas, most = std::max(1, (c.max_len + 255) / 256);
+  p.splits = int(std::max(1ll, std::min({want, most, (long long)kMostSplits})));
+  return p;
+}
+
 }  // namespace
 
-size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads) {
-  kv_check(c, head_dim);
+static void check_heads(const KvCacheView& c, int heads) {
   if (heads <= 0 || heads > 32768 || heads % c.kv_heads != 0) throw std::invalid_argument("kv attention: heads must be a multiple of kv_heads");
-  return 256;
+}
+
+size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads, int rows) {
+  kv_check(c, head_dim);
+  check_heads(c, heads);
+  if (rows <= 0) return 256;
+  const AttentionPlan p = plan_for(c, heads, rows);
+  return p.splits > 1 ? size_t(rows) * heads * p.splits * kPartFloats * sizeof(float) : 256;
 }
 
 void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
-  const size_t need = kv_attention_workspace_bytes(c, head_dim, g.heads);
+  kv_check(c, head_dim);
+  check_heads(c, g.heads);
   if (c.rows <= 0) return;
   if (!g.q || !g.out || !workspace) throw std::invalid_argument("kv attention: null operand");
-  if (workspace_bytes < need) throw std::invalid_argument("kv attention: workspace too small");
   if (g.ld_q < g.heads * kKvHeadDim || g.ld_out < g.heads * kKvHeadDim || g.ld_q % 8 != 0 || g.ld_out % 8 != 0 || !aligned16(g.q) || !aligned16(g.out))
     throw std::invalid_argument("kv attention: row pitches must cover heads * 128 columns and keep 16-byte alignment");
   if (g.q == g.out) throw std::invalid_argument("kv attention: out may not alias q");
+  if (workspace_bytes < 256 || !aligned16(workspace) || workspace_bytes < kv_attention_workspace_bytes(c, head_dim, g.heads, c.rows))
+    throw std::invalid_argument("kv attention: workspace too small or not 16-byte aligned");
   g.group = g.heads / c.kv_heads;
   g.scale_log2 = (scale > 0.0f ? scale : 0.08838834764831845f) * 1.4426950408889634f;
   c.status = device_status_word();
-  const long long units = ((long long)c.max_new * g.heads + kWarps - 1) / kWarps;
-  const cudaError_t e = launch_overlapped(0, kv_attention_kernel, dim3(unsigned(units < 65535 ? units : 65535), c.batch < 65535 ? c.batch : 65535), dim3(kWarps * 32), 0, stream, c, g);
+  const AttentionPlan p = plan_for(c, g.heads, c.rows);
+  float* parts = static_cast<float*>(workspace);
+  const dim3 grid(p.splits * p.col_tiles, c.kv_heads, std::min(c.batch, 65535));
+  cudaError_t e = launch_overlapped(0, p.nt == 1 ? kv_attention_kernel<1> : kv_attention_kernel<2>, grid, dim3(kThreads), 0, stream, c, g, parts, p.splits);
+  if (e == cudaSuccess && p.splits > 1) {
+    const long long units = ((long long)std::min(c.max_new, c.rows) * g.heads + kWarps - 1) / kWarps;
+    e = launch_overlapped(0, kv_join_kernel, dim3(unsigned(std::min(units, 65535ll)), std::min(c.batch, 65535)), dim3(kThreads), 0, stream, c, g,
+                          static_cast<const float*>(parts), p.splits);
+  }
   if (e != cudaSuccess) throw std::runtime_error(std::string("kv attention: launch failed: ") + cudaGetErrorString(e));
 }
 

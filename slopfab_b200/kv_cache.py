@@ -116,7 +116,7 @@ class KvCache:
             raise ValueError("out has as many rows as q")
         with on_device(self.device):
             desc, n = self._desc(s), C.c_size_t()
-            check(lib.sfq_kv_cache_attention_workspace_bytes(C.byref(desc), heads, C.byref(n)))
+            check(lib.sfq_kv_cache_attention_workspace_bytes(C.byref(desc), heads, rows, C.byref(n)))
             ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
             check(lib.sfq_kv_cache_attention(C.byref(desc), q.data_ptr(), ld, out.data_ptr(), ld_out, heads, rows, scale, ws.data_ptr(), n.value, stream_ptr()))
         return out

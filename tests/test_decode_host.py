@@ -75,7 +75,7 @@ def test_bad_caches_are_refused(over):
     assert _append(_cache(**over)) == sfq.ERR_INVALID_ARGUMENT
     assert _attend(_cache(**over)) == sfq.ERR_INVALID_ARGUMENT
     n = C.c_size_t()
-    assert sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache(**over)), 4, C.byref(n)) == sfq.ERR_INVALID_ARGUMENT
+    assert sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache(**over)), 4, 3, C.byref(n)) == sfq.ERR_INVALID_ARGUMENT
 
 
 @pytest.mark.parametrize("over", [dict(q=None), dict(q_out=None), dict(k=None), dict(v=None), dict(heads=-1), dict(ld_q=504), dict(ld_q=516),
@@ -93,7 +93,7 @@ def test_append_refuses_rotations(over):
 
 
 @pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(ws=None), dict(ws_bytes=0), dict(heads=0), dict(heads=3), dict(ld_q=504),
-                                  dict(ld_out=516), dict(out=A), dict(q=A + 8), dict(out=2 * A + 2)])
+                                  dict(ld_out=516), dict(out=A), dict(ws=A + 8), dict(q=A + 8), dict(out=2 * A + 2)])
 def test_attention_refuses_operands(over):
     assert _attend(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
 
@@ -101,7 +101,7 @@ def test_attention_refuses_operands(over):
 def test_no_rows_is_a_no_op_and_null_descriptors_are_refused():
     assert _append(_cache(), rows=0, q=None, k=None) == sfq.OK and _attend(_cache(), rows=0, q=None) == sfq.OK
     assert _append(None) == sfq.ERR_INVALID_ARGUMENT and _attend(None) == sfq.ERR_INVALID_ARGUMENT
-    assert sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache()), 4, None) == sfq.ERR_INVALID_ARGUMENT
+    assert sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache()), 4, 3, None) == sfq.ERR_INVALID_ARGUMENT
 
 
 def test_python_faces_refuse_what_does_not_fit():
