@@ -30,6 +30,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 64;        // tokens a warp takes at a time
 constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
 constexpr int kMostSplits = 64;
+constexpr int kResident[4] = {0, 3, 2, 2};  // CTAs of an SM, by the query tiles of eight
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -57,16 +58,35 @@ __device__ __forceinline__ uint4 load_cache(const uint8_t* p) {
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+// 2^x to two units in the last place of fp32; results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // 0xFF in the bytes of w that are NaN (0x7F or 0xFF).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
 
+// Notes for one channel that the columns which see a token with a NaN value there are NaN: `bad` has the bytes of tokens at ..
+// at + 3, column i sees the first `first + (col0 + i) / group` tokens.
+__device__ __noinline__ void note_nan(uint32_t* columns, uint32_t bad, int at, int first, int col0, int cols, int group) {
+  for (int i = 0; i < cols; ++i) {
+    const int sees = first + (col0 + i) / group;
+    for (int k = 0; k < 4; ++k)
+      if ((bad >> (8 * k) & 1) != 0 && at + k < sees) atomicOr(columns, 1u << i);
+  }
+}
+
 template <int NT>
-__global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
+__global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
   constexpr int kCols = NT * 8;
-  __shared__ float sh_o[kWarps][128 * (kCols + 1)];
+  extern __shared__ __align__(16) float sh_o[];  // [kWarps][128][kCols + 1]
   __shared__ float sh_m[kWarps][kCols], sh_mv[kWarps][kCols], sh_l[kWarps][kCols];
   __shared__ int sh_seen[kWarps][kCols];
   __shared__ uint2 sh_q[8][NT][32];
+  __shared__ uint32_t sh_nan[kKvHeadDim];  // columns that are NaN in a channel
+  static_assert(kKvHeadDim == kThreads, "a thread clears a channel");
   __shared__ float sh_qscale[kCols];
   grid_dependency_release();
   grid_dependency_wait();
@@ -82,6 +102,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
     const int all_cols = s.rows * g.group;
     for (int col0 = int(blockIdx.x) / splits * kCols; col0 < all_cols; col0 += int(gridDim.x) / splits * kCols) {
       __syncthreads();  // what the tile in front left in shared memory has been read
+      sh_nan[threadIdx.x] = 0;
       // ---- the queries as fp16, each times a power of two that takes its largest element just below 2^15. Its eight significant bits are
       // exact down to 2^-31 of that; what is smaller is off by 2^-39 of it at most.
       for (int i = threadIdx.x; i < kCols * 4; i += kThreads) {
@@ -147,9 +168,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
         const int t = tile * kTile + chunk * 16;
         return tile < tile_end && t < last ? kv_page(c, b, t >> c.page_shift) : -1;
       };
-      // One query tile has the registers for a tile's K under the products of the one in front.
-      constexpr bool kAhead = NT == 1;
-      uint4 kraw[kAhead ? 4 : 1][4];
       const uint8_t* k_at = c.k;
       int k_step = 0;
       auto seek_k = [&](int tile, int page) {
@@ -157,35 +175,20 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
         k_at = page < 0 ? c.k : c.k + (((size_t(page) * c.kv_heads + head) << c.page_shift) + slot + (gq & 1)) * kKvHeadDim + q * 16;
         k_step = page < 0 ? 0 : 1;  // a chunk that is not there: any bytes
       };
-      auto load_k = [&](int t, uint4 (&to)[4]) {
+      auto load_k = [&](int t, uint4 (&to)[4]) {  // rows of MMA t
 #pragma unroll
         for (int u = 0; u < 4; ++u) to[u] = load_cache(k_at + k_step * ((t * 4 + (u >> 1) * 2) * kKvHeadDim + (u & 1) * 64));
       };
-      auto load_ahead = [&](int tile, int page) {
-        seek_k(tile, page);
-        if constexpr (kAhead) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) load_k(t, kraw[t]);
-        }
-      };
+      uint4 kraw[2][4];
       int tile = split * per_split + warp;
       int page_k = page_of(tile, gq >> 1), page_v = page_of(tile, q);
       int next_k = page_of(tile + kWarps, gq >> 1), next_v = page_of(tile + kWarps, q);
-      if (tile < tile_end) load_ahead(tile, page_k);
+      if (tile < tile_end) {
+        seek_k(tile, page_k);
+        load_k(0, kraw[0]);
+      }
       for (; tile < tile_end; tile += kWarps) {
         const int t0 = tile * kTile;
-        // ---- V of this tile on its way
-        uint4 vraw[8][2];
-        auto load_v = [&] {
-          const int slot = (tile * kTile + q * 16) & page_mask;
-          const uint8_t* p = page_v < 0 ? c.v : c.v + (((size_t(page_v) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
-          const int step = page_v < 0 ? 0 : 8 << c.page_shift;
-#pragma unroll
-          for (int d = 0; d < 8; ++d)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) vraw[d][h] = load_cache(p + (d * 2 + h) * step);
-        };
-        if constexpr (kAhead) load_v();
         const float ks = page_k < 0 ? 0.0f : c.k_scale[size_t(page_k) * c.kv_heads + head];
         const float vs = page_k < 0 ? 0.0f : c.v_scale[size_t(page_k) * c.kv_heads + head];
         // ---- scores
@@ -194,44 +197,40 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int n = 0; n < NT; ++n) sc[t][n][0] = sc[t][n][1] = sc[t][n][2] = sc[t][n][3] = 0.0f;
-        if constexpr (kAhead) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (t < 3) load_k(t + 1, kraw[(t + 1) & 1]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            uint2 bq[NT];
+            uint32_t a0, a1, a2, a3;
+            e4m3_pairs(word_of(kraw[t & 1][j >> 2], j & 3), a0, a2);
+            e4m3_pairs(word_of(kraw[t & 1][2 + (j >> 2)], j & 3), a1, a3);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) bq[n] = sh_q[j][n][lane];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              uint32_t a0, a1, a2, a3;
-              e4m3_pairs(word_of(kraw[t][j >> 2], j & 3), a0, a2);
-              e4m3_pairs(word_of(kraw[t][2 + (j >> 2)], j & 3), a1, a3);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(sc[t][n], a0, a1, a2, a3, bq[n].x, bq[n].y);
+            for (int n = 0; n < NT; ++n) {
+              const uint2 bq = sh_q[j][n][lane];
+              mma_f16(sc[t][n], a0, a1, a2, a3, bq.x, bq.y);
             }
           }
-        } else {
-          uint4 two[2][4];
-          load_k(0, two[0]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            if (t < 3) load_k(t + 1, two[(t + 1) & 1]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint32_t a0, a1, a2, a3;
-              e4m3_pairs(word_of(two[t & 1][j >> 2], j & 3), a0, a2);
-              e4m3_pairs(word_of(two[t & 1][2 + (j >> 2)], j & 3), a1, a3);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint2 bq = sh_q[j][n][lane];
-                mma_f16(sc[t][n], a0, a1, a2, a3, bq.x, bq.y);
-              }
-            }
-          }
-          load_v();
         }
+        // ---- V of this tile in four parts of 32 channels, two of them on their way at a time
+        const uint8_t* v_at = c.v;
+        int v_step = 0;
+        if (page_v >= 0) {
+          const int slot = (tile * kTile + q * 16) & page_mask;
+          v_at = c.v + (((size_t(page_v) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
+          v_step = 8 << c.page_shift;
+        }
+        auto load_v = [&](int part, uint4 (&to)[2][2]) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) to[d][h] = load_cache(v_at + (part * 4 + d * 2 + h) * v_step);
+        };
+        uint4 vraw[2][2][2];
+        load_v(0, vraw[0]);
+        load_v(1, vraw[1]);
         const int page = page_k;
         page_k = next_k;
-        if (tile + kWarps < tile_end) load_ahead(tile + kWarps, page_k);
         // ---- weights
         const bool whole = __all_sync(0xffffffffu, page >= 0) && t0 + kTile <= min(first_hidden, length);
         const int mine = t0 + (gq >> 1) * 16 + (gq & 1);  // token of row gq of MMA 0; row gq + 8 is two behind, MMA t four t
@@ -278,8 +277,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float m_new = fmaxf(m[n][e], top[n][e]), mv_new = fmaxf(mv[n][e], top_v[n][e]);
-            l[n][e] *= m_new == -INFINITY ? 1.0f : exp2f(m[n][e] - m_new);  // exp2(-inf - x) = 0 on the first tile
-            keep[n][e] = mv_new == -INFINITY ? 1.0f : exp2f(mv[n][e] - mv_new);
+            l[n][e] *= m_new == -INFINITY ? 1.0f : exp2_fast(m[n][e] - m_new);  // exp2(-inf - x) = 0 on the first tile
+            keep[n][e] = mv_new == -INFINITY ? 1.0f : exp2_fast(mv[n][e] - mv_new);
             moved |= mv_new != mv[n][e];
             m[n][e] = m_new, mv[n][e] = mv_new;
           }
@@ -305,85 +304,57 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              l[n][e & 1] += exp2f(sc[t][n][e] - ref[e & 1]);
-              w[e] = exp2f(sc[t][n][e] + ref_v[e & 1]) * frac;
+              l[n][e & 1] += exp2_fast(sc[t][n][e] - ref[e & 1]);
+              w[e] = exp2_fast(sc[t][n][e] + ref_v[e & 1]) * frac;
             }
             p[t][n][0] = transpose8x8(half_pair(w[0], w[1]));
             p[t][n][1] = transpose8x8(half_pair(w[2], w[3]));
           }
         }
-        // ---- V behind the sequence's end, or of no page, is zeros: a weight of zero does not undo NaN bytes
         const int v0 = t0 + q * 16;
-        if (t0 + kTile > length || !__all_sync(0xffffffffu, page_v >= 0)) {
-          const int live = page_v < 0 ? 0 : max(0, min(16, length - v0));
+        const bool ragged = t0 + kTile > length || !__all_sync(0xffffffffu, page_v >= 0);
+        const bool hidden = t0 + kTile > first_hidden;
+        const int live = page_v < 0 ? 0 : max(0, min(16, length - v0));  // bytes of a channel that are tokens of this sequence
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int bytes = min(max(live - 4 * w, 0), 4);
-            const uint32_t mask = bytes == 4 ? 0xFFFFFFFFu : (1u << (8 * bytes)) - 1u;
+        for (int part = 0; part < 4; ++part) {
+          uint4(&v)[2][2] = vraw[part & 1];
+          if (ragged || hidden) {
+            // V behind the sequence's end, or of no page, is zeros: a weight of zero does not undo NaN bytes. Of tokens that some of the
+            // columns do not see, NaN bytes are taken out and noted for the columns that do.
 #pragma unroll
-            for (int d = 0; d < 8; ++d)
+            for (int w = 0; w < 4; ++w) {
+              const int bytes = min(max(live - 4 * w, 0), 4);
+              const uint32_t mask = bytes == 4 ? 0xFFFFFFFFu : (1u << (8 * bytes)) - 1u;
 #pragma unroll
-              for (int h = 0; h < 2; ++h) (w == 0 ? vraw[d][h].x : w == 1 ? vraw[d][h].y : w == 2 ? vraw[d][h].z : vraw[d][h].w) &= mask;
-          }
-        }
-        if (t0 + kTile > first_hidden) {
-          // Tokens that some of the columns do not see: NaN among their values may reach only those that do. They are taken out of V, and
-          // a product of their places with who sees what says where they belong.
-          uint32_t any = 0;
+              for (int d = 0; d < 2; ++d)
 #pragma unroll
-          for (int d = 0; d < 8; ++d)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) any |= nan_bytes(word_of(vraw[d][h], w));
-          if (__any_sync(0xffffffffu, any != 0)) {
-#pragma unroll 1
-            for (int n = 0; n < NT; ++n) {
-              const int sees_mine = min(length, past + min(col0 + n * 8 + gq, all_cols - 1) / g.group + 1);
-#pragma unroll
-              for (int d = 0; d < 8; ++d) {
-                float places[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                  uint32_t a[2][2], bsee[2];
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const uint32_t bad = nan_bytes(word_of(vraw[d][h], t)) & 0x38383838u;  // e4m3 1.0
-                    e4m3_pairs(bad, a[h][0], a[h][1]);
+                for (int h = 0; h < 2; ++h) {
+                  uint32_t& word = w == 0 ? v[d][h].x : w == 1 ? v[d][h].y : w == 2 ? v[d][h].z : v[d][h].w;
+                  word &= mask;
+                  const uint32_t bad = hidden ? nan_bytes(word) : 0;
+                  if (bad != 0) {
+                    note_nan(&sh_nan[part * 32 + d * 16 + h * 8 + gq], bad, v0 + w * 4, past + 1, col0, min(kCols, all_cols - col0), g.group);
+                    word &= ~bad;
                   }
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const int at = v0 + t * 4 + h * 2;
-                    bsee[h] = (at < sees_mine ? 0x3C00u : 0u) | (at + 1 < sees_mine ? 0x3C000000u : 0u);
-                  }
-                  mma_f16(places, a[0][0], a[1][0], a[0][1], a[1][1], bsee[0], bsee[1]);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                  for (int k = 0; k < NT; ++k)
-                    if (k == n && places[e] != 0.0f) o[d][k][e] = NAN;
-              }
             }
+          }
 #pragma unroll
-            for (int d = 0; d < 8; ++d)
+          for (int d = 0; d < 2; ++d)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                vraw[d][h].x &= ~nan_bytes(vraw[d][h].x), vraw[d][h].y &= ~nan_bytes(vraw[d][h].y);
-                vraw[d][h].z &= ~nan_bytes(vraw[d][h].z), vraw[d][h].w &= ~nan_bytes(vraw[d][h].w);
-              }
+            for (int t = 0; t < 4; ++t) {
+              uint32_t a0, a1, a2, a3;
+              e4m3_pairs(word_of(v[d][0], t), a0, a2);
+              e4m3_pairs(word_of(v[d][1], t), a1, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(o[part * 2 + d][n], a0, a1, a2, a3, p[t][n][0], p[t][n][1]);
+            }
+          if (part < 2) load_v(part + 2, v);
+          if (part == 2 && tile + kWarps < tile_end) {
+            seek_k(tile + kWarps, page_k);
+            load_k(0, kraw[0]);
           }
         }
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            uint32_t a0, a1, a2, a3;
-            e4m3_pairs(word_of(vraw[d][0], t), a0, a2);
-            e4m3_pairs(word_of(vraw[d][1], t), a1, a3);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(o[d][n], a0, a1, a2, a3, p[t][n][0], p[t][n][1]);
-          }
         page_v = next_v;
         next_k = page_of(tile + 2 * kWarps, gq >> 1), next_v = page_of(tile + 2 * kWarps, q);
       }
@@ -403,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sh_o[warp][(d * 16 + gq + (e >> 1) * 8) * (kCols + 1) + n * 8 + q * 2 + (e & 1)] = o[d][n][e];
+          for (int e = 0; e < 4; ++e) sh_o[(warp * kKvHeadDim + d * 16 + gq + (e >> 1) * 8) * (kCols + 1) + n * 8 + q * 2 + (e & 1)] = o[d][n][e];
       if (gq == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -425,11 +396,14 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
         for (int w = 0; w < kWarps; ++w) {
           if (sh_seen[w][col] == 0) continue;
           const float ref = mm == -INFINITY ? 0.0f : mm;
-          ll = fmaf(sh_l[w][col], sh_m[w][col] == -INFINITY && sh_l[w][col] == 0.0f ? 0.0f : exp2f(sh_m[w][col] - ref), ll);
-          const float f = sh_mv[w][col] == -INFINITY ? 1.0f : exp2f(sh_mv[w][col] - ref);  // a part without a finite score is 0 or NaN
+          ll = fmaf(sh_l[w][col], sh_m[w][col] == -INFINITY && sh_l[w][col] == 0.0f ? 0.0f : exp2_fast(sh_m[w][col] - ref), ll);
+          const float f = sh_mv[w][col] == -INFINITY ? 1.0f : exp2_fast(sh_mv[w][col] - ref);  // a part without a finite score is 0 or NaN
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sum[k] = fmaf(sh_o[w][(d4 + k) * (kCols + 1) + col], f, sum[k]);
+          for (int k = 0; k < 4; ++k) sum[k] = fmaf(sh_o[(w * kKvHeadDim + d4 + k) * (kCols + 1) + col], f, sum[k]);
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (sh_nan[d4 + k] >> col & 1) sum[k] = NAN;
         const int at = col0 + col, row = s.row0 + at / g.group, qh = head * g.group + at % g.group;
         if (splits > 1) {
           float* part = parts + ((size_t(row) * g.heads + qh) * splits + split) * kPartFloats;
@@ -447,31 +421,61 @@ __global__ void __launch_bounds__(kThreads, 2) kv_attention_kernel(KvCacheView c
   }
 }
 
-// One warp per row and head: its parts in order.
+// One CTA per row and head: its parts in order, a quarter of them a warp.
 __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvCacheView c, KvAttentionArgs g, const float* parts, int splits) {
+  __shared__ float4 sh_o[kWarps][32];
+  __shared__ float sh_l[kWarps];
   grid_dependency_release();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int b = blockIdx.y; b < c.batch; b += gridDim.y) {
     const KvSequence s = kv_sequence(c, b);
-    for (long long unit = (long long)blockIdx.x * kWarps + int(threadIdx.x >> 5); unit < (long long)s.rows * g.heads; unit += gridDim.x * kWarps) {
+    for (long long unit = blockIdx.x; unit < (long long)s.rows * g.heads; unit += gridDim.x) {
       const int row = s.row0 + int(unit / g.heads), qh = int(unit % g.heads);
       const float* part = parts + (size_t(row) * g.heads + qh) * splits * kPartFloats;
-      float mm = -INFINITY, ll = 0.0f, sum[4] = {0, 0, 0, 0};
+      static_assert(kMostSplits == 64, "two parts a lane");
+      float mm = -INFINITY, f[2];
       bool any = false;
-      for (int i = 0; i < splits; ++i) mm = fmaxf(mm, part[i * kPartFloats + 128]);
-      for (int i = 0; i < splits; ++i) {
-        const float4 st = *reinterpret_cast<const float4*>(part + i * kPartFloats + 128), o = *reinterpret_cast<const float4*>(part + i * kPartFloats + lane * 4);
-        if (st.z == 0.0f) continue;
-        any = true;
-        const float f = st.x == -INFINITY && st.y == 0.0f ? 0.0f : exp2f(st.x - (mm == -INFINITY ? 0.0f : mm));
-        ll = fmaf(st.y, f, ll);
-        sum[0] = fmaf(o.x, f, sum[0]), sum[1] = fmaf(o.y, f, sum[1]), sum[2] = fmaf(o.z, f, sum[2]), sum[3] = fmaf(o.w, f, sum[3]);
+      float4 st[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = lane + 32 * h;
+        st[h] = i < splits ? *reinterpret_cast<const float4*>(part + i * kPartFloats + 128) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        mm = fmaxf(mm, st[h].x), any |= st[h].z != 0.0f;
       }
-      const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;
-      __nv_bfloat162 lo = __floats2bfloat162_rn(sum[0] * inv, sum[1] * inv), hi = __floats2bfloat162_rn(sum[2] * inv, sum[3] * inv);
-      *reinterpret_cast<uint2*>(g.out + size_t(row) * g.ld_out + qh * kKvHeadDim + lane * 4) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+      any = __any_sync(0xffffffffu, any);
+      // a part without a finite score has weight 1: it is zeros, or NaN
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f[h] = st[h].x == -INFINITY ? 1.0f : exp2_fast(st[h].x - (mm == -INFINITY ? 0.0f : mm));
+      float ll = 0.0f;
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int each = (splits + kWarps - 1) / kWarps, end = min(splits, (warp + 1) * each);
+#pragma unroll 8
+      for (int i = warp * each; i < end; ++i) {
+        const float4 o = *reinterpret_cast<const float4*>(part + i * kPartFloats + lane * 4);
+        const float w = __shfl_sync(0xffffffffu, i < 32 ? f[0] : f[1], i & 31), li = __shfl_sync(0xffffffffu, i < 32 ? st[0].y : st[1].y, i & 31);
+        ll = fmaf(li, w, ll);
+        sum.x = fmaf(o.x, w, sum.x), sum.y = fmaf(o.y, w, sum.y), sum.z = fmaf(o.z, w, sum.z), sum.w = fmaf(o.w, w, sum.w);
+      }
+      __syncthreads();  // the row in front has been read
+      sh_o[warp][lane] = sum;
+      if (lane == 0) sh_l[warp] = ll;
+      __syncthreads();
+      if (warp == 0) {
+        ll = 0.0f;
+        sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 o = sh_o[w][lane];
+          ll += sh_l[w], sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
+        }
+        const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;
+        __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv), hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+        *reinterpret_cast<uint2*>(g.out + size_t(row) * g.ld_out + qh * kKvHeadDim + lane * 4) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
     }
   }
 }
@@ -486,10 +490,11 @@ struct AttentionPlan {
 AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
   AttentionPlan p;
   const long long cols = (long long)std::min(c.max_new, rows) * (heads / c.kv_heads);
-  p.nt = cols > 8 ? 2 : 1;
+  p.nt = cols > 16 ? 3 : cols > 8 ? 2 : 1;
   p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
   const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
-  const long long want = (4ll * device_sm_count() + ctas - 1) / ctas, most = std::max(1, (c.max_len + 255) / 256);
+  const int resident = kResident[p.nt] * device_sm_count();
+  const long long want = ctas < resident ? resident / ctas : 1, most = std::max(1, (c.max_len + 255) / 256);
   p.splits = int(std::max(1ll, std::min({want, most, (long long)kMostSplits})));
   return p;
 }
@@ -524,9 +529,12 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   const AttentionPlan p = plan_for(c, g.heads, c.rows);
   float* parts = static_cast<float*>(workspace);
   const dim3 grid(p.splits * p.col_tiles, c.kv_heads, std::min(c.batch, 65535));
-  cudaError_t e = launch_overlapped(0, p.nt == 1 ? kv_attention_kernel<1> : kv_attention_kernel<2>, grid, dim3(kThreads), 0, stream, c, g, parts, p.splits);
+  const size_t smem = size_t(kWarps) * kKvHeadDim * (p.nt * 8 + 1) * sizeof(float);
+  const auto kernel = p.nt == 1 ? kv_attention_kernel<1> : p.nt == 2 ? kv_attention_kernel<2> : kv_attention_kernel<3>;
+  reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "kv attention");
+  cudaError_t e = launch_overlapped(0, kernel, grid, dim3(kThreads), smem, stream, c, g, parts, p.splits);
   if (e == cudaSuccess && p.splits > 1) {
-    const long long units = ((long long)std::min(c.max_new, c.rows) * g.heads + kWarps - 1) / kWarps;
+    const long long units = (long long)std::min(c.max_new, c.rows) * g.heads;
     e = launch_overlapped(0, kv_join_kernel, dim3(unsigned(std::min(units, 65535ll)), std::min(c.batch, 65535)), dim3(kThreads), 0, stream, c, g,
                           static_cast<const float*>(parts), p.splits);
   }
