@@ -518,7 +518,8 @@ SFQ_API int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rot
 /* out[rows, heads * 128] = softmax(q K^T scale) V over the cache: the i-th of a sequence's n new tokens sees its first length - n + i + 1
  * keys; query head h reads kv head h / (heads / kv_heads). scale <= 0 selects 1 / sqrt(128). A row that sees no key is zero; a NaN or +inf
  * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Slots behind a sequence's length may hold
- * anything. The workspace is scratch of one call; it needs no initialisation. */
+ * anything. The workspace is scratch of one call and needs no initialisation; it may be null where
+ * sfq_kv_cache_attention_workspace_bytes gives 0. */
 SFQ_API int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, int rows, size_t* out);
 SFQ_API int sfq_kv_cache_attention(const sfq_kv_cache* cache, const void* d_q_bf16, int ld_q, void* d_out_bf16, int ld_out, int heads,
                                    int rows, float scale, void* d_workspace, size_t workspace_bytes, void* stream);

@@ -30,6 +30,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 64;        // tokens a warp takes at a time
 constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
 constexpr int kMostSplits = 64;
+constexpr int kSms = 148;        // the launch is planned for; the workspace can be asked for without a device
 constexpr int kResident[4] = {0, 3, 2, 2};  // CTAs of an SM, by the query tiles of eight
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -493,7 +494,7 @@ AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
   p.nt = cols > 16 ? 3 : cols > 8 ? 2 : 1;
   p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
   const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
-  const int resident = kResident[p.nt] * device_sm_count();
+  const int resident = kResident[p.nt] * kSms;
   const long long want = ctas < resident ? resident / ctas : 1, most = std::max(1, (c.max_len + 255) / 256);
   p.splits = int(std::max(1ll, std::min({want, most, (long long)kMostSplits})));
   return p;
@@ -508,20 +509,21 @@ static void check_heads(const KvCacheView& c, int heads) {
 size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads, int rows) {
   kv_check(c, head_dim);
   check_heads(c, heads);
-  if (rows <= 0) return 256;
+  if (rows <= 0) return 0;
   const AttentionPlan p = plan_for(c, heads, rows);
-  return p.splits > 1 ? size_t(rows) * heads * p.splits * kPartFloats * sizeof(float) : 256;
+  return p.splits > 1 ? size_t(rows) * heads * p.splits * kPartFloats * sizeof(float) : 0;
 }
 
 void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   kv_check(c, head_dim);
   check_heads(c, g.heads);
   if (c.rows <= 0) return;
-  if (!g.q || !g.out || !workspace) throw std::invalid_argument("kv attention: null operand");
+  if (!g.q || !g.out) throw std::invalid_argument("kv attention: null operand");
   if (g.ld_q < g.heads * kKvHeadDim || g.ld_out < g.heads * kKvHeadDim || g.ld_q % 8 != 0 || g.ld_out % 8 != 0 || !aligned16(g.q) || !aligned16(g.out))
     throw std::invalid_argument("kv attention: row pitches must cover heads * 128 columns and keep 16-byte alignment");
   if (g.q == g.out) throw std::invalid_argument("kv attention: out may not alias q");
-  if (workspace_bytes < 256 || !aligned16(workspace) || workspace_bytes < kv_attention_workspace_bytes(c, head_dim, g.heads, c.rows))
+  const size_t need = kv_attention_workspace_bytes(c, head_dim, g.heads, c.rows);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
     throw std::invalid_argument("kv attention: workspace too small or not 16-byte aligned");
   g.group = g.heads / c.kv_heads;
   g.scale_log2 = (scale > 0.0f ? scale : 0.08838834764831845f) * 1.4426950408889634f;

@@ -6,8 +6,8 @@ from dataclasses import dataclass
 
 import torch
 
-from . import KvCacheDesc, RotaryDesc, check, lib, ptr, stream_ptr
-from .linear import on_device
+from . import KvCacheDesc, RotaryDesc, check, lib, ptr
+from .linear import on_device, raw_stream
 
 HEAD_DIM = 128
 
@@ -21,6 +21,10 @@ class Sequences:
     row_start: torch.Tensor
     max_new: int
     max_len: int
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, "_checked", None)  # what was found about the fields so far
+        object.__setattr__(self, name, value)
 
 
 @dataclass
@@ -62,7 +66,7 @@ class KvCache:
         if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
             raise ValueError("the pools and their scales lie on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.kv_heads, self.device = kv_heads, k.device
+        self.kv_heads, self.device, self._device = kv_heads, k.device, k.get_device()
         self._pool = (ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, page_size, kv_heads, dim)
 
     @staticmethod
@@ -72,51 +76,58 @@ class KvCache:
         return KvCache(k, v, *(torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)))
 
     def _desc(self, s: Sequences) -> KvCacheDesc:
-        t = s.page_table
-        if t.dtype != torch.int32 or s.seq_len.dtype != torch.int32 or s.row_start.dtype != torch.int32:
+        t, n, r = s.page_table, s.seq_len, s.row_start
+        at = (self._pool, t.data_ptr(), n.data_ptr(), r.data_ptr())
+        if s._checked is not None and s._checked[0] == at:
+            return s._checked[1]
+        if t.dtype != torch.int32 or n.dtype != torch.int32 or r.dtype != torch.int32:
             raise ValueError("page_table, seq_len and row_start must be int32")
         batch, max_pages = t.shape
-        if s.seq_len.shape != (batch,) or s.row_start.shape != (batch + 1,):
-            raise ValueError("seq_len has an entry per sequence, row_start one more")
-        if not t.device == s.seq_len.device == s.row_start.device == self.device:
+        if n.shape != (batch,) or r.shape != (batch + 1,) or not (t.is_contiguous() and n.is_contiguous() and r.is_contiguous()):
+            raise ValueError("seq_len has an entry per sequence, row_start one more; all are contiguous")
+        if not t.get_device() == n.get_device() == r.get_device() == self._device:
             raise ValueError("the sequences' tensors lie on the cache's device")
-        return KvCacheDesc(*self._pool, ptr(t), ptr(s.seq_len), ptr(s.row_start), batch, max_pages, s.max_new, s.max_len)
+        desc = KvCacheDesc(*self._pool, *at[1:], batch, max_pages, s.max_new, s.max_len)
+        object.__setattr__(s, "_checked", (at, desc))
+        return desc
 
-    def _rows(self, name: str, t: torch.Tensor, cols: int) -> int:
-        if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[1] != cols or t.stride(1) != 1 or t.device != self.device:
-            raise ValueError(f"{name} must be bf16 [rows, {cols}] with contiguous rows, on the cache's device")
-        return t.stride(0)
+    def _pitch(self, name: str, t: torch.Tensor, rows: int | None, cols: int) -> int:
+        shape, stride = t.shape, t.stride()
+        if t.dtype != torch.bfloat16 or len(shape) != 2 or shape[1] != cols or stride[1] != 1 or t.get_device() != self._device or rows not in (None, shape[0]):
+            raise ValueError(f"{name} must be bf16 [{'rows' if rows is None else rows}, {cols}] with contiguous rows, on the cache's device")
+        return max(stride[0], cols)  # a single row may have any stride
 
     def append(self, s: Sequences, qkv: torch.Tensor, heads: int, q_out: torch.Tensor | None = None, rotary: Rotary | None = None) -> torch.Tensor:
         """Stores k and v of the fused projection qkv [rows, (heads + 2 kv_heads) * 128] and returns q, normed and rotated
         (q_out [rows, heads * 128]; pass a view of qkv's first columns to have it in place)."""
-        ld, rows = self._rows("qkv", qkv, (heads + 2 * self.kv_heads) * HEAD_DIM), qkv.shape[0]
+        ld, rows = self._pitch("qkv", qkv, None, (heads + 2 * self.kv_heads) * HEAD_DIM), qkv.shape[0]
         if q_out is None:
             q_out = torch.empty((rows, heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
-        ld_out = self._rows("q_out", q_out, heads * HEAD_DIM)
-        if q_out.shape[0] != rows:
-            raise ValueError("q_out has as many rows as qkv")
+        ld_out = self._pitch("q_out", q_out, rows, heads * HEAD_DIM)
         if rotary is not None and rotary.position is not None and rotary.position.shape != (rows,):
             raise ValueError("position has an entry per row")
         q = qkv.data_ptr()
         k = q + heads * HEAD_DIM * 2
-        with on_device(self.device):
-            check(lib.sfq_kv_cache_append(C.byref(self._desc(s)), C.byref(rotary.desc) if rotary is not None else None, q, ld, q_out.data_ptr(), ld_out,
-                                          heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, stream_ptr()))
+        with on_device(self._device):
+            status = lib.sfq_kv_cache_append(C.byref(self._desc(s)), C.byref(rotary.desc) if rotary is not None else None, q, ld, q_out.data_ptr(), ld_out,
+                                             heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, raw_stream(self._device))
+        if status:
+            check(status)
         return q_out
 
     def attention(self, s: Sequences, q: torch.Tensor, heads: int, out: torch.Tensor | None = None, scale: float = 0.0) -> torch.Tensor:
         """softmax(q K^T scale) V of the new tokens' q [rows, heads * 128] over the cache, causal among them; scale 0 means 1 / sqrt(128).
         The workspace is the call's own, so that calls on several streams and captured graphs share none."""
-        ld, rows = self._rows("q", q, heads * HEAD_DIM), q.shape[0]
+        ld, rows = self._pitch("q", q, None, heads * HEAD_DIM), q.shape[0]
         if out is None:
             out = torch.empty((rows, heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
-        ld_out = self._rows("out", out, heads * HEAD_DIM)
-        if out.shape[0] != rows:
-            raise ValueError("out has as many rows as q")
-        with on_device(self.device):
+        ld_out = self._pitch("out", out, rows, heads * HEAD_DIM)
+        with on_device(self._device):
             desc, n = self._desc(s), C.c_size_t()
             check(lib.sfq_kv_cache_attention_workspace_bytes(C.byref(desc), heads, rows, C.byref(n)))
-            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
-            check(lib.sfq_kv_cache_attention(C.byref(desc), q.data_ptr(), ld, out.data_ptr(), ld_out, heads, rows, scale, ws.data_ptr(), n.value, stream_ptr()))
+            ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
+            status = lib.sfq_kv_cache_attention(C.byref(desc), q.data_ptr(), ld, out.data_ptr(), ld_out, heads, rows, scale, ws.data_ptr() if n.value else None,
+                                                n.value, raw_stream(self._device))
+        if status:
+            check(status)
         return out

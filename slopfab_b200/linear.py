@@ -20,29 +20,32 @@ def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
     return s.cuda_stream
 
 
-def on_device(device: torch.device):
-    """Makes the device of a call's tensors current for it, at no cost where it is already."""
-    if device.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, not on {device}")
-    return _SAME if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def on_device(index: int):
+    """Makes device `index` current for a call, at no cost where it is already."""
+    if index < 0:
+        raise ValueError("tensors must be on a CUDA device")
+    return _SAME if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 _SAME = contextlib.nullcontext()
+raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device, without the Python object
 
 
 def linear_matvec(w: QuantWeight, x: torch.Tensor, y: torch.Tensor | None = None, activation: int = ACT_NONE) -> torch.Tensor:
     """y = act(x W^T + b) for the few rows of a decoding step, the NVFP4 or NF4 weight read as stored (sfq_linear_matvec).
     x: bf16 [rows, in]; y: bf16 [rows, out], out / 2 columns with ACT_SWIGLU. Runs on x's device and its current stream."""
     cols = w.out_features // 2 if activation == ACT_SWIGLU else w.out_features
-    if x.dim() != 2 or x.shape[1] != w.in_features or x.dtype != torch.bfloat16:
-        raise ValueError(f"x must be bf16 [rows, {w.in_features}]")
-    rows, device = x.shape[0], x.device
+    if x.dim() != 2 or x.shape[1] != w.in_features or x.dtype != torch.bfloat16 or not x.is_contiguous():
+        raise ValueError(f"x must be contiguous bf16 [rows, {w.in_features}]")
+    rows, device = x.shape[0], x.get_device()
     if y is None:
-        y = torch.empty((rows, cols), dtype=torch.bfloat16, device=device)
-    elif y.shape != (rows, cols) or y.dtype != torch.bfloat16 or y.device != device:
-        raise ValueError(f"y must be bf16 [{rows}, {cols}] on x's device")
+        y = torch.empty((rows, cols), dtype=torch.bfloat16, device=x.device)
+    elif y.shape != (rows, cols) or y.dtype != torch.bfloat16 or y.get_device() != device or not y.is_contiguous():
+        raise ValueError(f"y must be contiguous bf16 [{rows}, {cols}] on x's device")
     with on_device(device):
-        check(lib.sfq_linear_matvec(C.byref(w), ptr(x), rows, activation, ptr(y), stream_ptr()))
+        status = lib.sfq_linear_matvec(C.byref(w), x.data_ptr(), rows, activation, y.data_ptr(), raw_stream(device))
+    if status:
+        check(status)
     return y
 
 

@@ -92,10 +92,21 @@ def test_append_refuses_rotations(over):
     assert _append(_cache(), rotary=sfq.RotaryDesc(**f)) == sfq.ERR_INVALID_ARGUMENT
 
 
-@pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(ws=None), dict(ws_bytes=0), dict(heads=0), dict(heads=3), dict(ld_q=504),
-                                  dict(ld_out=516), dict(out=A), dict(ws=A + 8), dict(q=A + 8), dict(out=2 * A + 2)])
+@pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(heads=0), dict(heads=3), dict(ld_q=504),
+                                  dict(ld_out=516), dict(out=A), dict(q=A + 8), dict(out=2 * A + 2)])
 def test_attention_refuses_operands(over):
     assert _attend(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
+
+
+def test_attention_refuses_workspaces():
+    long = _cache(max_len=100000)  # divided: parts are kept
+    n = C.c_size_t()
+    sfq.check(sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(long), 4, 3, C.byref(n)))
+    assert n.value > 0
+    for over in (dict(ws=None), dict(ws=A + 8), dict(ws_bytes=0), dict(ws_bytes=n.value - 1)):
+        assert _attend(long, **over) == sfq.ERR_INVALID_ARGUMENT and b"workspace" in sfq.lib.sfq_last_error()
+    sfq.check(sfq.lib.sfq_kv_cache_attention_workspace_bytes(C.byref(_cache()), 4, 3, C.byref(n)))
+    assert n.value == 0
 
 
 def test_no_rows_is_a_no_op_and_null_descriptors_are_refused():

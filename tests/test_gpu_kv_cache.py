@@ -225,6 +225,26 @@ def test_nan_and_infinity():
     assert bool(got[1].isnan().all()) and torch.equal(got[0], clean[0])
 
 
+def test_nan_of_a_later_token_stays_hidden():
+    """Among a sequence's new tokens, a NaN in one's k or v reaches it and those behind it, in that channel, and none in front."""
+    counts, lens = [40, 9], [100, 200]
+    c = Case(counts, lens, 1, 3, 32, seed=21).fill(lens)
+    q = c.q()
+    clean = c.check_attention(q)
+    t = 85  # the 26th of sequence 0's new tokens
+    i, o = int(c.table[0, t // 32]), t % 32
+    was = c.cache.v[i, 0, 77, o].clone()
+    c.cache.v[i, 0, 77, o] = 0xFF
+    got = c.cache.attention(c.seqs, q, 3).view(-1, 3, D)
+    want = clean.view(-1, 3, D).clone()
+    want[25:40, :, 77] = float("nan")
+    assert torch.equal(got.nan_to_num(1e4), want.nan_to_num(1e4))
+    c.cache.v[i, 0, 77, o] = was
+    c.cache.k[i, 0, o, 5] = 0x7F
+    got = c.cache.attention(c.seqs, q, 3)
+    assert bool(got[25:40].isnan().all()) and torch.equal(got[:25], clean[:25]) and torch.equal(got[40:], clean[40:])
+
+
 def test_entries_that_make_no_sense_are_reported_and_not_followed():
     counts, lens = [1, 2, 1, 1], [100, 70, 40, 90]
     c = Case(counts, lens, 2, 2, 32, seed=11).fill(lens)
