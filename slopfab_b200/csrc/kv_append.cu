@@ -19,12 +19,12 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kLanes = 16;                  // threads of one head's vector, 8 channels each
 constexpr int kAtOnce = kThreads / kLanes;  // vectors a block works on at once
-constexpr int kQueryHeads = 8;              // query heads a block of the page form rotates
+constexpr int kQueryHeads = 4;              // query heads a block of the page form rotates
 constexpr int kFewTokens = 4;               // new tokens of a sequence up to which a warp takes a (page, head)
-constexpr int kHeld = 4;                    // vectors a thread of the page form holds between its two passes
+constexpr int kHeld = 2;                    // vectors a thread of the page form holds between its two passes
 
 // A thread's eight channels of a head lie in two pieces of four: with rotation over 2 h channels, 4 l .. and h + 4 l .. for the first
 // h / 4 threads, so that both halves of a pair are in one thread, and eight neighbours for the others.
@@ -210,12 +210,15 @@ __global__ void __launch_bounds__(128) kv_append_few_kernel(KvCacheView c, Rotar
 // Prompts. blockIdx.x: page of the sequence's new tokens; y: sequence; z: a kv head, behind them groups of query heads. A thread takes the
 // same piece of up to kHeld tokens' vectors, which stay in registers while the block finds the page's scale (pages of more than 64 tokens
 // are computed twice); V goes through shared memory, so that a channel's tokens are stored side by side.
-__global__ void __launch_bounds__(kThreads) kv_append_page_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
+__global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
   grid_dependency_release();
   grid_dependency_wait();
   __shared__ float peaks[2][kThreads / 32];
-  extern __shared__ __align__(16) uint8_t sh_v[];  // [128][page_size + 16]
-  const int page_size = 1 << c.page_shift, pitch = page_size + 16;
+  // V's codes, a channel's tokens side by side. A word more than they take, and two more every 32 channels, puts the words that the
+  // sixteen threads of a vector write to into different banks.
+  extern __shared__ __align__(16) uint8_t sh_v[];
+  const int page_size = 1 << c.page_shift;
+  auto staged = [&](int channel) { return sh_v + channel * (page_size + 4) + (channel >> 5) * 8; };
   const int vector = threadIdx.x / kLanes, l = threadIdx.x & 15;
   const Place at = place_of(rot, l);
   const bool queries = int(blockIdx.z) >= c.kv_heads;
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_page_kernel(KvCacheView c,
             *reinterpret_cast<uint32_t*>(kc + size_t(run.slot0 + j) * kKvHeadDim + at.b) = encode4(k[h] + 4, inv_k);
             const uint32_t lo = encode4(x, inv_v), hi = encode4(x + 4, inv_v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sh_v[(l * 8 + e) * pitch + run.slot0 + j] = uint8_t((e < 4 ? lo : hi) >> (8 * (e & 3)));
+            for (int e = 0; e < 8; ++e) staged(l * 8 + e)[run.slot0 + j] = uint8_t((e < 4 ? lo : hi) >> (8 * (e & 3)));
           }
         }
       __syncthreads();  // every thread has read the old scales, too
@@ -323,10 +326,11 @@ __global__ void __launch_bounds__(kThreads) kv_append_page_kernel(KvCacheView c,
       const int first = run.slot0, end = run.slot0 + run.tokens, groups = page_size / 16;
       for (int i = threadIdx.x; i < kKvHeadDim * groups; i += kThreads) {
         const int channel = i / groups, t = i % groups * 16;
-        const uint8_t* from = sh_v + channel * pitch + t;
+        const uint8_t* from = staged(channel) + t;
         uint8_t* to = vc + (size_t(channel) << c.page_shift) + t;
         if (t >= first && t + 16 <= end) {
-          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+          const uint32_t* f = reinterpret_cast<const uint32_t*>(from);
+          *reinterpret_cast<uint4*>(to) = make_uint4(f[0], f[1], f[2], f[3]);
         } else {
           for (int k2 = max(first - t, 0); k2 < min(end - t, 16); ++k2) to[k2] = from[k2];
         }
@@ -370,7 +374,7 @@ void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendA
     const int units = c.kv_heads + (g.heads + 1) / 2;
     e = launch_overlapped(bytes, kv_append_few_kernel, dim3((units + 3) / 4, pages, std::min(c.batch, 65535)), dim3(128), 0, stream, c, rot, g);
   } else {
-    const size_t smem = size_t(kKvHeadDim) * (page_size + 16);
+    const size_t smem = size_t(kKvHeadDim) * (page_size + 4) + 32;
     const int groups = (g.heads + kQueryHeads - 1) / kQueryHeads;
     e = launch_overlapped(bytes, kv_append_page_kernel, dim3(pages, std::min(c.batch, 65535), c.kv_heads + groups), dim3(kThreads), smem, stream, c, rot, g);
   }

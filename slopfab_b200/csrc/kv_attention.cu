@@ -4,8 +4,9 @@
 // half an instruction away from fp16. The products run on mma.sync m16n8k16, transposed, so that the query heads of a group (and the new
 // tokens of a sequence), of which there are few, are its N of 8 and the cache its M of 16:
 //   S^T [tokens, queries] = K Q^T    O^T [channels, queries] += V^T P^T
-// A warp takes 64 tokens at a time. V lies with a channel's tokens side by side, so both operands are 16-byte loads straight into
-// registers, and the weights P go from the first product's result to the second one's operand by 8 x 8 transposes between lanes. Which
+// A warp takes 64 tokens at a time, which asynchronous copies put into its own 16 KB of shared memory: the next K while this one's softmax
+// and second product run, the next V under the scores. V lies with a channel's tokens side by side, so both operands are 16-byte reads, and
+// the weights P go from the first product's result to the second one's operand by 8 x 8 transposes between lanes. Which
 // token is which row of the first product is free: the order is chosen so that the transposed weights of four MMAs meet the 16
 // neighbouring tokens of a lane's V. Softmax with running maximum and sum in fp32; the page's scale of K goes into the score, that of V into
 // the weight.
@@ -28,6 +29,7 @@ using namespace ptx;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 64;        // tokens a warp takes at a time
+constexpr int kTileBytes = kTile * kKvHeadDim;  // of K, and of V
 constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
 constexpr int kMostSplits = 64;
 constexpr int kSms = 148;        // the launch is planned for; the workspace can be asked for without a device
@@ -52,11 +54,16 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint4 load_cache(const uint8_t* p) {
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // 16 bytes, or zeros for bytes == 0
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // 2^x to two units in the last place of fp32; results below 2^-126 are zero.
@@ -82,7 +89,10 @@ __device__ __noinline__ void note_nan(uint32_t* columns, uint32_t bad, int at, i
 template <int NT>
 __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
   constexpr int kCols = NT * 8;
-  extern __shared__ __align__(16) float sh_o[];  // [kWarps][128][kCols + 1]
+  // a tile of K [64 tokens][128] and of V [128][64 tokens] for each warp; when they are done, [kWarps][128][kCols + 1] sums
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* const sh_o = reinterpret_cast<float*>(smem);
+  static_assert(kWarps * kKvHeadDim * (kCols + 1) * 4 <= kWarps * 2 * kTileBytes, "the sums fit");
   __shared__ float sh_m[kWarps][kCols], sh_mv[kWarps][kCols], sh_l[kWarps][kCols];
   __shared__ int sh_seen[kWarps][kCols];
   __shared__ uint2 sh_q[8][NT][32];
@@ -164,74 +174,87 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.0f;
 
-      // K is read by the lane whose rows lie in chunk gq / 2 of the tile's four chunks of 16 tokens, V in chunk q.
-      auto page_of = [&](int tile, int chunk) -> int {
-        const int t = tile * kTile + chunk * 16;
+      // A tile's pages: lane c holds that of chunk c % 4 of its four chunks of 16 tokens, -1 where there is none.
+      auto page_of = [&](int tile) -> int {
+        const int t = tile * kTile + q * 16;
         return tile < tile_end && t < last ? kv_page(c, b, t >> c.page_shift) : -1;
       };
-      const uint8_t* k_at = c.k;
-      int k_step = 0;
-      auto seek_k = [&](int tile, int page) {
-        const int slot = (tile * kTile + (gq >> 1) * 16) & page_mask;
-        k_at = page < 0 ? c.k : c.k + (((size_t(page) * c.kv_heads + head) << c.page_shift) + slot + (gq & 1)) * kKvHeadDim + q * 16;
-        k_step = page < 0 ? 0 : 1;  // a chunk that is not there: any bytes
-      };
-      auto load_k = [&](int t, uint4 (&to)[4]) {  // rows of MMA t
+      const uint32_t k_sh = smem_u32(smem) + warp * 2 * kTileBytes, v_sh = k_sh + kTileBytes;
+      // K: 16 bytes of four tokens at a time, the unit exclusive-or'ed with four times the token's last bit, so that the two rows that eight
+      // lanes read together lie in different banks. V: 16 tokens of eight channels at a time. Chunks without a page are zeros.
+      auto fetch_k = [&](int tile, int pages) {
+        if (tile < tile_end) {
+          const int unit = lane & 7, token0 = lane >> 3;
+          const uint32_t to = k_sh + token0 * 128 + ((unit ^ ((token0 & 1) << 2)) << 4);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) to[u] = load_cache(k_at + k_step * ((t * 4 + (u >> 1) * 2) * kKvHeadDim + (u & 1) * 64));
+          for (int chunk = 0; chunk < 4; ++chunk) {
+            const int page = __shfl_sync(0xffffffffu, pages, chunk);
+            const int slot = (tile * kTile + chunk * 16) & page_mask;
+            const uint8_t* from = page < 0 ? c.k : c.k + (((size_t(page) * c.kv_heads + head) << c.page_shift) + slot + token0) * kKvHeadDim + unit * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cp_async16(to + (chunk * 16 + i * 4) * 128, from + (page < 0 ? 0 : i * 4 * kKvHeadDim), page < 0 ? 0 : 16);
+          }
+        }
+        cp_commit();
       };
-      uint4 kraw[2][4];
+      auto fetch_v = [&](int tile, int pages) {
+        if (tile < tile_end) {
+          const int slot = (tile * kTile + q * 16) & page_mask;
+          const uint8_t* from = pages < 0 ? c.v : c.v + (((size_t(pages) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
+          const int step = pages < 0 ? 0 : 8 << c.page_shift;
+          const uint32_t to = v_sh + gq * 64 + q * 16;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) cp_async16(to + i * 8 * 64, from + i * step, pages < 0 ? 0 : 16);
+        }
+        cp_commit();
+      };
       int tile = split * per_split + warp;
-      int page_k = page_of(tile, gq >> 1), page_v = page_of(tile, q);
-      int next_k = page_of(tile + kWarps, gq >> 1), next_v = page_of(tile + kWarps, q);
-      if (tile < tile_end) {
-        seek_k(tile, page_k);
-        load_k(0, kraw[0]);
-      }
+      int pages = page_of(tile), next_pages = page_of(tile + kWarps);
+      fetch_k(tile, pages);
+      fetch_v(tile, pages);
       for (; tile < tile_end; tile += kWarps) {
         const int t0 = tile * kTile;
-        const float ks = page_k < 0 ? 0.0f : c.k_scale[size_t(page_k) * c.kv_heads + head];
-        const float vs = page_k < 0 ? 0.0f : c.v_scale[size_t(page_k) * c.kv_heads + head];
+        const size_t block = size_t(max(pages, 0)) * c.kv_heads + head;
+        const float ks_mine = pages < 0 ? 0.0f : c.k_scale[block], vs_mine = pages < 0 ? 0.0f : c.v_scale[block];
         // ---- scores
+        cp_wait<1>();
+        __syncwarp();
         float sc[4][NT][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) sc[t][n][0] = sc[t][n][1] = sc[t][n][2] = sc[t][n][3] = 0.0f;
-#pragma unroll
         for (int t = 0; t < 4; ++t) {
-          if (t < 3) load_k(t + 1, kraw[(t + 1) & 1]);
+          uint4 k[2][2];  // [row gq or gq + 8][half of the channels]
+          const int token = (gq >> 1) * 16 + t * 4 + (gq & 1);
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) k[r][u] = lds128(k_sh + (token + 2 * r) * 128 + (((u * 4 + q) ^ ((gq & 1) << 2)) << 4));
+          float odd[NT][4];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][n][e] = odd[n][e] = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             uint32_t a0, a1, a2, a3;
-            e4m3_pairs(word_of(kraw[t & 1][j >> 2], j & 3), a0, a2);
-            e4m3_pairs(word_of(kraw[t & 1][2 + (j >> 2)], j & 3), a1, a3);
+            e4m3_pairs(word_of(k[0][j >> 2], j & 3), a0, a2);
+            e4m3_pairs(word_of(k[1][j >> 2], j & 3), a1, a3);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint2 bq = sh_q[j][n][lane];
-              mma_f16(sc[t][n], a0, a1, a2, a3, bq.x, bq.y);
+              mma_f16(j & 1 ? odd[n] : sc[t][n], a0, a1, a2, a3, bq.x, bq.y);
             }
           }
-        }
-        // ---- V of this tile in four parts of 32 channels, two of them on their way at a time
-        const uint8_t* v_at = c.v;
-        int v_step = 0;
-        if (page_v >= 0) {
-          const int slot = (tile * kTile + q * 16) & page_mask;
-          v_at = c.v + (((size_t(page_v) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
-          v_step = 8 << c.page_shift;
-        }
-        auto load_v = [&](int part, uint4 (&to)[2][2]) {
 #pragma unroll
-          for (int d = 0; d < 2; ++d)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) to[d][h] = load_cache(v_at + (part * 4 + d * 2 + h) * v_step);
-        };
-        uint4 vraw[2][2][2];
-        load_v(0, vraw[0]);
-        load_v(1, vraw[1]);
+            for (int e = 0; e < 4; ++e) sc[t][n][e] += odd[n][e];
+        }
+        __syncwarp();
+        fetch_k(tile + kWarps, next_pages);
+        // this lane's rows lie in chunk gq / 2
+        const int page_k = __shfl_sync(0xffffffffu, pages, gq >> 1), page_v = pages;
+        const float ks = __shfl_sync(0xffffffffu, ks_mine, gq >> 1), vs = __shfl_sync(0xffffffffu, vs_mine, gq >> 1);
         const int page = page_k;
-        page_k = next_k;
         // ---- weights
         const bool whole = __all_sync(0xffffffffu, page >= 0) && t0 + kTile <= min(first_hidden, length);
         const int mine = t0 + (gq >> 1) * 16 + (gq & 1);  // token of row gq of MMA 0; row gq + 8 is two behind, MMA t four t
@@ -315,10 +338,16 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
         const int v0 = t0 + q * 16;
         const bool ragged = t0 + kTile > length || !__all_sync(0xffffffffu, page_v >= 0);
         const bool hidden = t0 + kTile > first_hidden;
+        cp_wait<1>();
+        __syncwarp();
         const int live = page_v < 0 ? 0 : max(0, min(16, length - v0));  // bytes of a channel that are tokens of this sequence
 #pragma unroll
         for (int part = 0; part < 4; ++part) {
-          uint4(&v)[2][2] = vraw[part & 1];
+          uint4 v[2][2];
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) v[d][h] = lds128(v_sh + (part * 32 + d * 16 + h * 8 + gq) * 64 + q * 16);
           if (ragged || hidden) {
             // V behind the sequence's end, or of no page, is zeros: a weight of zero does not undo NaN bytes. Of tokens that some of the
             // columns do not see, NaN bytes are taken out and noted for the columns that do.
@@ -350,15 +379,14 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
 #pragma unroll
               for (int n = 0; n < NT; ++n) mma_f16(o[part * 2 + d][n], a0, a1, a2, a3, p[t][n][0], p[t][n][1]);
             }
-          if (part < 2) load_v(part + 2, v);
-          if (part == 2 && tile + kWarps < tile_end) {
-            seek_k(tile + kWarps, page_k);
-            load_k(0, kraw[0]);
-          }
         }
-        page_v = next_v;
-        next_k = page_of(tile + 2 * kWarps, gq >> 1), next_v = page_of(tile + 2 * kWarps, q);
+        __syncwarp();
+        fetch_v(tile + kWarps, next_pages);
+        pages = next_pages;
+        next_pages = page_of(tile + 2 * kWarps);
       }
+      cp_wait<0>();
+      __syncthreads();  // every warp's tiles have been read
 
       // ---- the four warps joined
 #pragma unroll
@@ -495,7 +523,9 @@ AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
   p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
   const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
   const int resident = kResident[p.nt] * kSms;
-  const long long want = ctas < resident ? resident / ctas : 1, most = std::max(1, (c.max_len + 255) / 256);
+  // Few sequences: as many CTAs as run at once. More: twice as many, so that unequal lengths even out. A part of less than 256 tokens
+  // (a tile for each warp) is not worth its joining.
+  const long long want = 4 * ctas <= resident ? resident / ctas : (2 * resident + ctas - 1) / ctas, most = std::max(1, c.max_len / (4 * ctas <= resident ? 256 : 768));
   p.splits = int(std::max(1ll, std::min({want, most, (long long)kMostSplits})));
   return p;
 }
@@ -531,7 +561,7 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   const AttentionPlan p = plan_for(c, g.heads, c.rows);
   float* parts = static_cast<float*>(workspace);
   const dim3 grid(p.splits * p.col_tiles, c.kv_heads, std::min(c.batch, 65535));
-  const size_t smem = size_t(kWarps) * kKvHeadDim * (p.nt * 8 + 1) * sizeof(float);
+  const size_t smem = size_t(kWarps) * 2 * kTileBytes;
   const auto kernel = p.nt == 1 ? kv_attention_kernel<1> : p.nt == 2 ? kv_attention_kernel<2> : kv_attention_kernel<3>;
   reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "kv attention");
   cudaError_t e = launch_overlapped(0, kernel, grid, dim3(kThreads), smem, stream, c, g, parts, p.splits);
