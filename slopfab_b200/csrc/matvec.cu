@@ -197,18 +197,18 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
   const int last_group = g.in / 64 - 1;
   uint32_t absmax_byte[MT];
   float absmax_outer[MT], absmax[MT];
-  size_t absmax_row[MT];  // its row's first element
+  uint32_t absmax_row[MT];  // its row's first group of 64
   auto seek_absmax = [&](int unit) {
     if constexpr (NF4) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) absmax_row[m] = size_t(weight_row<true>(unit * MT + m, lane >> 1, g.out, swiglu)) * g.in;
+      for (int m = 0; m < MT; ++m) absmax_row[m] = uint32_t(weight_row<true>(unit * MT + m, lane >> 1, g.out, swiglu)) * uint32_t(last_group + 1);
     }
   };
   auto fetch_absmax = [&](int s) {
     if constexpr (NF4) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const size_t block = (absmax_row[m] + uint32_t(min(s * 2 + (lane & 1), last_group)) * 64) >> g.block_shift;
+        const uint32_t block = (absmax_row[m] + uint32_t(min(s * 2 + (lane & 1), last_group))) >> (g.block_shift - 6);
         absmax_byte[m] = g.scale[block], absmax_outer[m] = g.nested_absmax[block >> g.nested_shift];
       }
     }
@@ -229,32 +229,46 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
   auto stage_x = [&](int band) {  // band < 0: the first attempt
     const int units = steps * kStep / 8;
     const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x3400), __ushort_as_bfloat16(0x3400));  // 2^-23
+    const __nv_bfloat162 sixty_four = __halves2bfloat162(__ushort_as_bfloat16(0x4280), __ushort_as_bfloat16(0x4280));
     const __nv_bfloat162 zero = __halves2bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
     uint32_t low = 0;
     __nv_bfloat162 top = zero;
-    for (int r = 0; r < g.rows; ++r) {
-      const __nv_bfloat16* row = g.x + size_t(r) * g.in;
-      for (int k8 = threadIdx.x; k8 < units; k8 += kThreads) {
-        const uint4 raw = k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(row + k8 * 8) : make_uint4(0, 0, 0, 0);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    constexpr int kBatch = 4;  // loads in flight
+    int r = 0, k8 = threadIdx.x;
+    while (k8 >= units) k8 -= units, ++r;
+    while (r < g.rows) {
+      uint4 raw[kBatch];
+      int rr[kBatch], kk[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        rr[i] = r, kk[i] = k8;
+        raw[i] = r < g.rows && k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(g.x + size_t(r) * g.in + k8 * 8) : make_uint4(0, 0, 0, 0);
+        k8 += kThreads;
+        while (k8 >= units) k8 -= units, ++r;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (rr[i] >= g.rows) break;
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float even = __uint_as_float(w[i] << 16), odd = __uint_as_float(w[i] & 0xFFFF0000u);
+        for (int j = 0; j < 4; ++j) {
+          float even, odd;
           if (band < 0) {
-            const uint32_t mag = w[i] & 0x7FFF7FFFu;
+            const uint32_t mag = w[j] & 0x7FFF7FFFu;
             const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&mag);
             low |= __hlt2_mask(a, least) & __hgt2_mask(a, zero);
             top = __hmax2(top, a);
-            even *= 64.0f, odd *= 64.0f;
+            const __nv_bfloat162 up = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[j]), sixty_four);  // exact
+            even = __low2float(up), odd = __high2float(up);
           } else {
-            even = banded(even, row_e[r], band), odd = banded(odd, row_e[r], band);
+            even = banded(__uint_as_float(w[j] << 16), row_e[rr[i]], band), odd = banded(__uint_as_float(w[j] & 0xFFFF0000u), row_e[rr[i]], band);
           }
-          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(even), "f"(odd));
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[j]) : "f"(even), "f"(odd));
         }
-        const int step = k8 >> 4;
-        const int piece = NF4 ? ((k8 >> 3) & 1) * 2 + (k8 & 1) : k8 & 3, quarter = NF4 ? (k8 >> 1) & 3 : (k8 >> 2) & 3;
-        *reinterpret_cast<uint4*>(smem + p.x_off + (((step * 4 + piece) * g.rows + r) * 4 + quarter) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        const int step = kk[i] >> 4;
+        const int piece = NF4 ? ((kk[i] >> 3) & 1) * 2 + (kk[i] & 1) : kk[i] & 3, quarter = NF4 ? (kk[i] >> 1) & 3 : (kk[i] >> 2) & 3;
+        *reinterpret_cast<uint4*>(smem + p.x_off + (((step * 4 + piece) * g.rows + rr[i]) * 4 + quarter) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
     if (band < 0 && (low != 0 || fmaxf(__low2float(top), __high2float(top)) >= 1024.0f)) flags = 1;
@@ -379,7 +393,12 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
   };
 
   // The team's sums of a unit, added in the order of its warps, finished and stored.
-  float* const part = reinterpret_cast<float*>(smem + p.part_off) + team * kTeamWarps * MT * 16 * kPitch;
+  // NF4 keeps them in the unused halves of the table's lines.
+  const int part0 = team * kTeamWarps * MT * 16 * kPitch;
+  auto part = [&](int i) -> float& {
+    const int at = part0 + i;
+    return *reinterpret_cast<float*>(smem + (NF4 ? (at >> 5) * 256 + 128 + (at & 31) * 4 : p.part_off + at * 4));
+  };
   const int cols = swiglu ? g.out / 2 : g.out;
   auto finish = [&](int unit) {
     named_barrier(team + 1, kTeamWarps * 32);  // the sums of the unit in front have been read
@@ -388,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part[(warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)] = acc[m][n][e];
+        for (int e = 0; e < 4; ++e) part((warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)) = acc[m][n][e];
     named_barrier(team + 1, kTeamWarps * 32);
     const int per_tile = swiglu ? 8 : 16;
     for (int i = warp * 32 + lane; i < MT * per_tile * g.rows; i += kTeamWarps * 32) {
@@ -399,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
       for (int h = 0; h < (swiglu ? 2 : 1); ++h) {
         float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kTeamWarps; ++w) s += part[(w * MT * 16 + m * 16 + j + 8 * h) * kPitch + r];
+        for (int w = 0; w < kTeamWarps; ++w) s += part((w * MT * 16 + m * 16 + j + 8 * h) * kPitch + r);
         const int at = n + h * cols;
         const float b = g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
         z[h] = ldexpf(s * g.global_scale, row_e[r] - 14) + b;
@@ -487,7 +506,11 @@ template <bool NF4, int NT, int MT, int D> size_t plan(const MatvecArgs& g, int 
   p.ring_off = int(at);
   at += size_t(kTeams) * kTeamWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
   p.part_off = int(at);
-  at += size_t(kTeams) * kTeamWarps * MT * 16 * (NT * 8 + 1) * 4;
+  const size_t sums = size_t(kTeams) * kTeamWarps * MT * 16 * (NT * 8 + 1) * 4;
+  if (!NF4)
+    at += sums;
+  else if (sums > kTableBytes / 2)
+    return ~size_t(0);
   p.x_off = int(at);
   return at + size_t((g.in + kStep - 1) / kStep * kStep) * rows * 2;
 }
@@ -520,8 +543,8 @@ template <bool NF4> void launch_rows(MatvecArgs g, int cols, cudaStream_t stream
       launch<NF4, 2, 1, 2>(g, stream);
     else if (g.rows <= 2 && fits<NF4, 1, 1, 4>(g, g.rows))
       launch<NF4, 1, 1, 4>(g, stream);
-    else if (fits<NF4, 1, 2, 3>(g, g.rows) && g.out >= 32 * kTeams * device_sm_count())
-      launch<NF4, 1, 2, 3>(g, stream);
+    else if (fits<NF4, 1, 2, NF4 ? 2 : 3>(g, g.rows) && g.out >= 32 * kTeams * device_sm_count())
+      launch<NF4, 1, 2, NF4 ? 2 : 3>(g, stream);
     else if (fits<NF4, 1, 1, 4>(g, g.rows))
       launch<NF4, 1, 1, 4>(g, stream);
     else
@@ -542,6 +565,7 @@ void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream
     if (!g.scale || !g.map || !g.nested_map || !g.nested_absmax) throw std::invalid_argument("matvec: nf4 weight without complete double-quant state");
     if (!power_of_two(nf4_block) || nf4_block < 64 || !power_of_two(nf4_nested_block)) throw std::invalid_argument("matvec: nf4 blocks must be powers of two, of 64 elements at least");
     if (g.in % 64 != 0) throw std::invalid_argument("matvec: nf4 needs in_features % 64 == 0");
+    if ((size_t(g.out) * g.in) >> 38 != 0) throw std::invalid_argument("matvec: nf4 weight of more than 2^38 elements");
     g.block_shift = log2_of(nf4_block), g.nested_shift = log2_of(nf4_nested_block);
     g.global_scale = 1.0f;
   } else {
