@@ -30,11 +30,14 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTeams = 2, kTeamWarps = 8, kThreads = kTeams * kTeamWarps * 32;
+constexpr int kTeamWarps = 8;
 constexpr size_t kMostSmem = 229376;  // dynamic; the kernel has about 2 KB of its own
 constexpr int kMostRows = 16;      // rows of x in one launch
 constexpr int kStep = 128;         // elements of K a warp takes at a time
 constexpr int kTableBytes = 65536; // NF4: entry of byte b for lane l at b * 256 + l * 4
+
+// Floats of a row of a warp's sums: one more than it has, against bank conflicts, where there is room.
+__host__ __device__ constexpr int sum_pitch(bool nf4, int nt) { return nt * 8 + (nf4 && nt == 2 ? 0 : 1); }
 
 struct Plan {
   int units = 0;  // groups of MT tiles of 16 weight rows
@@ -133,12 +136,12 @@ __device__ __forceinline__ float banded(float f, int e, int band) {
   return ldexpf(f, 14 - e + 32 * band);
 }
 
-template <bool NF4, int NT, int MT, int D>
-__global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_kernel(MatvecArgs g, Plan p) {
+template <bool NF4, int NT, int MT, int D, int TEAMS>
+__global__ void __launch_bounds__(TEAMS * kTeamWarps * 32, (!NF4 && D == 4) ? 2 : 1) matvec_kernel(MatvecArgs g, Plan p) {
+  constexpr int kThreads = TEAMS * kTeamWarps * 32;
   constexpr int kStage = MT * 1024 + (NF4 ? 0 : MT * 128);  // codes [MT][16 rows][64 bytes], scales [MT][2 slabs][16 rows][4 bytes]
-  constexpr int kPitch = NT * 8 + 1;
+  constexpr int kPitch = sum_pitch(NF4, NT);
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t flags;
   __shared__ int row_e[kMostRows], row_low[kMostRows];
   __shared__ float nested_map[NF4 ? 256 : 1];
   const int warp = (threadIdx.x >> 5) % kTeamWarps, team = threadIdx.x / (kTeamWarps * 32), lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
   const int steps = (g.in + kStep - 1) / kStep;
   const uint32_t base = smem_u32(smem);
   const uint32_t ring = base + p.ring_off + (threadIdx.x >> 5) * D * kStage;
-  const int first_unit = team * gridDim.x + blockIdx.x, all_teams = gridDim.x * kTeams;  // what is left over falls on different CTAs
+  const int first_unit = team * gridDim.x + blockIdx.x, all_teams = gridDim.x * TEAMS;  // what is left over falls on different CTAs
   grid_dependency_release();
 
   // The copies under way: the next one is step `fs` of unit `fu`.
@@ -226,14 +229,14 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
 
   // x [rows, in] as fp16: 16 bytes of eight elements, pairs with the odd element in the low half, at unit
   // ((step * 4 + piece) * rows + row) * 4 + lane % 4, which is the order in which the MMAs' lanes read them.
-  auto stage_x = [&](int band) {  // band < 0: the first attempt
+  auto stage_x = [&](int band) -> bool {  // band < 0: the first attempt; true where an element does not fit it
     const int units = steps * kStep / 8;
     const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x3400), __ushort_as_bfloat16(0x3400));  // 2^-23
     const __nv_bfloat162 sixty_four = __halves2bfloat162(__ushort_as_bfloat16(0x4280), __ushort_as_bfloat16(0x4280));
     const __nv_bfloat162 zero = __halves2bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
     uint32_t low = 0;
     __nv_bfloat162 top = zero;
-    constexpr int kBatch = 4;  // loads in flight
+    constexpr int kBatch = (!NF4 && D == 4) || TEAMS > 2 ? 4 : 8;  // loads in flight
     int r = 0, k8 = threadIdx.x;
     while (k8 >= units) k8 -= units, ++r;
     while (r < g.rows) {
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
         *reinterpret_cast<uint4*>(smem + p.x_off + (((step * 4 + piece) * g.rows + rr[i]) * 4 + quarter) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
-    if (band < 0 && (low != 0 || fmaxf(__low2float(top), __high2float(top)) >= 1024.0f)) flags = 1;
+    return low != 0 || fmaxf(__low2float(top), __high2float(top)) >= 1024.0f;
   };
 
   // Lanes of columns that stand for no row of x read another row's; what they add up is not stored.
@@ -312,11 +315,10 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
           }
         }
       }
-    } else {
+    } else {  // a group past the end of a row: x is zeros, the codes are, too, and the absmax is the last group's
       const uint32_t lane4 = lane * 4;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if (s * 2 + c > last_group) break;
         uint4 xv[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -429,22 +431,21 @@ __global__ void __launch_bounds__(kThreads, (!NF4 && D == 4) ? 2 : 1) matvec_ker
 
   grid_dependency_wait();
   start(first_unit, p.units);
-  if (threadIdx.x == 0) flags = 0;
   if (threadIdx.x < kMostRows) row_e[threadIdx.x] = kFixedExponent;
+  const float map = NF4 ? g.map[lane & 15] : 0.0f, nested = NF4 ? g.nested_map[threadIdx.x & 255] : 0.0f;
+  const bool misfit = stage_x(-1);
   if constexpr (NF4) {
-    // the table: two threads build the entry of a byte, odd element (low nibble) in the low half, and its 32 copies
-    const uint32_t b = threadIdx.x & 255;
-    const __half2 pair = __floats2half2_rn(g.map[b & 15], g.map[b >> 4]);
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(&pair);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(smem + b * 256 + ((i * 2 + (threadIdx.x >> 8) + b) & 7) * 16) = make_uint4(v, v, v, v);
-    if (threadIdx.x < 256) nested_map[b] = g.nested_map[b];
+    // the table: the entry of a byte, odd element (low nibble) in the low half, and its 32 copies
+    for (uint32_t i = threadIdx.x; i < 256 * 8; i += kThreads) {  // whole warps
+      const uint32_t b = i >> 3;
+      const __half2 pair = __floats2half2_rn(__shfl_sync(0xffffffffu, map, b & 15), __shfl_sync(0xffffffffu, map, b >> 4));
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(&pair);
+      *reinterpret_cast<uint4*>(smem + b * 256 + (i & 7) * 16) = make_uint4(v, v, v, v);
+    }
+    if (threadIdx.x < 256) nested_map[threadIdx.x] = nested;
   }
-  __syncthreads();  // flags
-  stage_x(-1);
-  __syncthreads();
   int bands = 0;
-  if (flags != 0) {
+  if (__syncthreads_or(misfit)) {
     // Each row's largest exponent and lowest band, over its finite elements that are not zero.
     for (int r = threadIdx.x >> 5; r < g.rows; r += kThreads / 32) {
       int most = -1000, least = 1000;
@@ -498,15 +499,15 @@ bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // What a launch with this kernel takes of shared memory for `rows` rows of x.
-template <bool NF4, int NT, int MT, int D> size_t plan(const MatvecArgs& g, int rows, Plan& p) {
+template <bool NF4, int NT, int MT, int D, int TEAMS> size_t plan(const MatvecArgs& g, int rows, Plan& p) {
   const bool swiglu = g.act == SFQ_ACT_SWIGLU;
   const int tiles = NF4 ? ((swiglu ? g.out / 2 : g.out) + (swiglu ? 7 : 15)) / (swiglu ? 8 : 16) : g.out / 16;
   p.units = (tiles + MT - 1) / MT;
   size_t at = NF4 ? kTableBytes : 0;
   p.ring_off = int(at);
-  at += size_t(kTeams) * kTeamWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
+  at += size_t(TEAMS) * kTeamWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
   p.part_off = int(at);
-  const size_t sums = size_t(kTeams) * kTeamWarps * MT * 16 * (NT * 8 + 1) * 4;
+  const size_t sums = size_t(TEAMS) * kTeamWarps * MT * 16 * sum_pitch(NF4, NT) * 4;
   if (!NF4)
     at += sums;
   else if (sums > kTableBytes / 2)
@@ -515,40 +516,40 @@ template <bool NF4, int NT, int MT, int D> size_t plan(const MatvecArgs& g, int 
   return at + size_t((g.in + kStep - 1) / kStep * kStep) * rows * 2;
 }
 
-template <bool NF4, int NT, int MT, int D> bool fits(const MatvecArgs& g, int rows) {
+template <bool NF4, int NT, int MT, int D, int TEAMS> bool fits(const MatvecArgs& g, int rows) {
   Plan p;
-  return plan<NF4, NT, MT, D>(g, rows, p) <= kMostSmem;
+  return plan<NF4, NT, MT, D, TEAMS>(g, rows, p) <= kMostSmem;
 }
 
-template <bool NF4, int NT, int MT, int D> void launch(const MatvecArgs& g, cudaStream_t stream) {
+template <bool NF4, int NT, int MT, int D, int TEAMS> void launch(const MatvecArgs& g, cudaStream_t stream) {
   Plan p;
-  const size_t bytes = plan<NF4, NT, MT, D>(g, g.rows, p);
-  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT, D>), bytes, "matvec");
+  const size_t bytes = plan<NF4, NT, MT, D, TEAMS>(g, g.rows, p);
+  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT, D, TEAMS>), bytes, "matvec");
   const int resident = !NF4 && D == 4 && bytes <= kMostSmem / 2 - 1024 ? 2 : 1;
-  const int ctas = std::min((p.units + kTeams - 1) / kTeams, resident * device_sm_count());
-  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT, D>, dim3(ctas), dim3(kThreads), bytes, stream, g, p);
+  const int ctas = std::min(p.units, resident * device_sm_count());
+  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT, D, TEAMS>, dim3(ctas), dim3(TEAMS * kTeamWarps * 32), bytes, stream, g, p);
   if (e != cudaSuccess) throw std::runtime_error(std::string("matvec: launch failed: ") + cudaGetErrorString(e));
 }
 
 template <bool NF4> void launch_rows(MatvecArgs g, int cols, cudaStream_t stream) {
-  if (!fits<NF4, 1, 1, 2>(g, 1)) throw std::invalid_argument("matvec: in_features too large");
+  constexpr int F = NF4 ? 3 : 2;  // teams
+  constexpr int DF = NF4 ? 3 : 4;
+  if (!fits<NF4, 1, 1, 2, 2>(g, 1)) throw std::invalid_argument("matvec: in_features too large");
   int rows = g.rows;
   while (rows > 0) {
     // as many rows at a time as x fits into shared memory for, in equal parts
     int most = std::min(rows, kMostRows);
-    while (most > 1 && !(most > 8 ? fits<NF4, 2, 1, 2>(g, most) : fits<NF4, 1, 1, 2>(g, most))) --most;
+    while (most > 1 && !(most > 8 ? fits<NF4, 2, 1, 2, 2>(g, most) : fits<NF4, 1, 1, 2, 2>(g, most))) --most;
     const int parts = (rows + most - 1) / most;
     g.rows = (rows + parts - 1) / parts;
     if (g.rows > 8)
-      launch<NF4, 2, 1, 2>(g, stream);
-    else if (g.rows <= 2 && fits<NF4, 1, 1, 4>(g, g.rows))
-      launch<NF4, 1, 1, 4>(g, stream);
-    else if (fits<NF4, 1, 2, NF4 ? 2 : 3>(g, g.rows) && g.out >= 32 * kTeams * device_sm_count())
-      launch<NF4, 1, 2, NF4 ? 2 : 3>(g, stream);
-    else if (fits<NF4, 1, 1, 4>(g, g.rows))
-      launch<NF4, 1, 1, 4>(g, stream);
+      launch<NF4, 2, 1, 2, 2>(g, stream);
+    else if (g.rows > (NF4 ? 4 : 2) && fits<NF4, 1, 2, NF4 ? 2 : 3, 2>(g, g.rows) && g.out >= 32 * 2 * device_sm_count())
+      launch<NF4, 1, 2, NF4 ? 2 : 3, 2>(g, stream);
+    else if (fits<NF4, 1, 1, DF, F>(g, g.rows))
+      launch<NF4, 1, 1, DF, F>(g, stream);
     else
-      launch<NF4, 1, 1, 2>(g, stream);
+      launch<NF4, 1, 1, 2, 2>(g, stream);
     rows -= g.rows;
     g.x += size_t(g.rows) * g.in;
     g.y += size_t(g.rows) * cols;
