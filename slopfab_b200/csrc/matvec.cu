@@ -10,8 +10,7 @@
 //   - NF4: a byte is looked up as two fp16 (the table's entries rounded by 2^-11) in a table of all 256 bytes that has a copy for each
 //     lane's bank; the absmax of 64 elements scales the fp32 sum of their four MMAs.
 //   - x becomes fp16 times a power of two for each row, exactly: see stage_x.
-// CTAs stay for the whole launch, so that x is made fp16 once per SM. Each has two teams of eight warps; a team takes 16 MT weight rows at
-// a time, its warps take turns along K in steps of 128, each with its own ring of asynchronous copies that runs on into the next rows, and
+// CTAs stay for the whole launch, so that x is made fp16 once per SM. Their warps form teams; a team takes 16 MT weight rows at a time, its warps take turns along K in steps of 128, each with its own ring of asynchronous copies that runs on into the next rows, and
 // their sums meet in shared memory in a fixed order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,7 +29,6 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTeamWarps = 8;
 constexpr size_t kMostSmem = 229376;  // dynamic; the kernel has about 2 KB of its own
 constexpr int kMostRows = 16;      // rows of x in one launch
 constexpr int kStep = 128;         // elements of K a warp takes at a time
@@ -136,9 +134,9 @@ __device__ __forceinline__ float banded(float f, int e, int band) {
   return ldexpf(f, 14 - e + 32 * band);
 }
 
-template <bool NF4, int NT, int MT, int D, int TEAMS>
-__global__ void __launch_bounds__(TEAMS * kTeamWarps * 32, (!NF4 && D == 4) ? 2 : 1) matvec_kernel(MatvecArgs g, Plan p) {
-  constexpr int kThreads = TEAMS * kTeamWarps * 32;
+template <bool NF4, int NT, int MT, int D, int WARPS, int kTeamWarps>
+__global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_kernel(MatvecArgs g, Plan p) {
+  constexpr int kThreads = WARPS * 32, TEAMS = WARPS / kTeamWarps;
   constexpr int kStage = MT * 1024 + (NF4 ? 0 : MT * 128);  // codes [MT][16 rows][64 bytes], scales [MT][2 slabs][16 rows][4 bytes]
   constexpr int kPitch = sum_pitch(NF4, NT);
   extern __shared__ __align__(128) uint8_t smem[];
@@ -236,7 +234,7 @@ __global__ void __launch_bounds__(TEAMS * kTeamWarps * 32, (!NF4 && D == 4) ? 2 
     const __nv_bfloat162 zero = __halves2bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
     uint32_t low = 0;
     __nv_bfloat162 top = zero;
-    constexpr int kBatch = (!NF4 && D == 4) || TEAMS > 2 ? 4 : 8;  // loads in flight
+    constexpr int kBatch = (!NF4 && D == 4) || WARPS > 16 ? 4 : 8;  // loads in flight
     int r = 0, k8 = threadIdx.x;
     while (k8 >= units) k8 -= units, ++r;
     while (r < g.rows) {
@@ -499,15 +497,15 @@ bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // What a launch with this kernel takes of shared memory for `rows` rows of x.
-template <bool NF4, int NT, int MT, int D, int TEAMS> size_t plan(const MatvecArgs& g, int rows, Plan& p) {
+template <bool NF4, int NT, int MT, int D, int WARPS> size_t plan(const MatvecArgs& g, int rows, Plan& p) {
   const bool swiglu = g.act == SFQ_ACT_SWIGLU;
   const int tiles = NF4 ? ((swiglu ? g.out / 2 : g.out) + (swiglu ? 7 : 15)) / (swiglu ? 8 : 16) : g.out / 16;
   p.units = (tiles + MT - 1) / MT;
   size_t at = NF4 ? kTableBytes : 0;
   p.ring_off = int(at);
-  at += size_t(TEAMS) * kTeamWarps * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
+  at += size_t(WARPS) * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
   p.part_off = int(at);
-  const size_t sums = size_t(TEAMS) * kTeamWarps * MT * 16 * sum_pitch(NF4, NT) * 4;
+  const size_t sums = size_t(WARPS) * MT * 16 * sum_pitch(NF4, NT) * 4;
   if (!NF4)
     at += sums;
   else if (sums > kTableBytes / 2)
@@ -516,40 +514,56 @@ template <bool NF4, int NT, int MT, int D, int TEAMS> size_t plan(const MatvecAr
   return at + size_t((g.in + kStep - 1) / kStep * kStep) * rows * 2;
 }
 
-template <bool NF4, int NT, int MT, int D, int TEAMS> bool fits(const MatvecArgs& g, int rows) {
+template <bool NF4, int NT, int MT, int D, int WARPS> bool fits(const MatvecArgs& g, int rows) {
   Plan p;
-  return plan<NF4, NT, MT, D, TEAMS>(g, rows, p) <= kMostSmem;
+  return plan<NF4, NT, MT, D, WARPS>(g, rows, p) <= kMostSmem;
 }
 
-template <bool NF4, int NT, int MT, int D, int TEAMS> void launch(const MatvecArgs& g, cudaStream_t stream) {
-  Plan p;
-  const size_t bytes = plan<NF4, NT, MT, D, TEAMS>(g, g.rows, p);
-  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT, D, TEAMS>), bytes, "matvec");
-  const int resident = !NF4 && D == 4 && bytes <= kMostSmem / 2 - 1024 ? 2 : 1;
+template <bool NF4, int NT, int MT, int D, int WARPS, int TEAM> void launch_team(const MatvecArgs& g, const Plan& p, size_t bytes, int resident, cudaStream_t stream) {
+  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT, D, WARPS, TEAM>), bytes, "matvec");
   const int ctas = std::min(p.units, resident * device_sm_count());
-  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT, D, TEAMS>, dim3(ctas), dim3(TEAMS * kTeamWarps * 32), bytes, stream, g, p);
+  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT, D, WARPS, TEAM>, dim3(ctas), dim3(WARPS * 32), bytes, stream, g, p);
   if (e != cudaSuccess) throw std::runtime_error(std::string("matvec: launch failed: ") + cudaGetErrorString(e));
 }
 
+// Teams of eight warps, or of four where that takes no more steps: a warp then walks longer rows of steps and fewer sums are joined.
+// 1 x 5120 -> 15360 NVFP4 13.4 us with eight, 12.1 with four; NF4 3 x 13824 -> 5120, where eight take half the steps, 21.4 against 24.4.
+template <bool NF4, int NT, int MT, int D, int WARPS> void launch(const MatvecArgs& g, cudaStream_t stream) {
+  Plan p;
+  const size_t bytes = plan<NF4, NT, MT, D, WARPS>(g, g.rows, p);
+  const int resident = !NF4 && D == 4 && bytes <= kMostSmem / 2 - 1024 ? 2 : 1;
+  const int steps = (g.in + kStep - 1) / kStep, sms = resident * device_sm_count();
+  auto cost = [&](int team) {
+    const int teams = WARPS / team * sms;
+    return ((p.units + teams - 1) / teams) * ((steps + team - 1) / team);
+  };
+  if (cost(4) <= cost(8))
+    launch_team<NF4, NT, MT, D, WARPS, 4>(g, p, bytes, resident, stream);
+  else
+    launch_team<NF4, NT, MT, D, WARPS, 8>(g, p, bytes, resident, stream);
+}
+
 template <bool NF4> void launch_rows(MatvecArgs g, int cols, cudaStream_t stream) {
-  constexpr int F = NF4 ? 3 : 2;  // teams
-  constexpr int DF = NF4 ? 3 : 4;
-  if (!fits<NF4, 1, 1, 2, 2>(g, 1)) throw std::invalid_argument("matvec: in_features too large");
+  if (!fits<NF4, 1, 1, 2, 16>(g, 1)) throw std::invalid_argument("matvec: in_features too large");
   int rows = g.rows;
   while (rows > 0) {
     // as many rows at a time as x fits into shared memory for, in equal parts
     int most = std::min(rows, kMostRows);
-    while (most > 1 && !(most > 8 ? fits<NF4, 2, 1, 2, 2>(g, most) : fits<NF4, 1, 1, 2, 2>(g, most))) --most;
+    while (most > 1 && !(most > 8 ? fits<NF4, 2, 1, 2, 16>(g, most) : fits<NF4, 1, 1, 2, 16>(g, most))) --most;
     const int parts = (rows + most - 1) / most;
     g.rows = (rows + parts - 1) / parts;
+    // Two tiles a step share the reads of x. NVFP4 needs them from three rows of x on and has two CTAs an SM below that; NF4, bound by its
+    // table's lookups, is better off with 24 warps up to four rows (3 x 13824 -> 5120 21.4 us; 16 warps 26.3; with two tiles, 16 rows
+    // 5120 -> 13824 35.0 against 37.5).
+    constexpr int kTwoTiles = NF4 ? 2 : 3;  // ring stages
     if (g.rows > 8)
-      launch<NF4, 2, 1, 2, 2>(g, stream);
-    else if (g.rows > (NF4 ? 4 : 2) && fits<NF4, 1, 2, NF4 ? 2 : 3, 2>(g, g.rows) && g.out >= 32 * 2 * device_sm_count())
-      launch<NF4, 1, 2, NF4 ? 2 : 3, 2>(g, stream);
-    else if (fits<NF4, 1, 1, DF, F>(g, g.rows))
-      launch<NF4, 1, 1, DF, F>(g, stream);
+      launch<NF4, 2, 1, 2, 16>(g, stream);
+    else if (g.rows > (NF4 ? 4 : 2) && fits<NF4, 1, 2, kTwoTiles, 16>(g, g.rows) && g.out >= 64 * device_sm_count())
+      launch<NF4, 1, 2, kTwoTiles, 16>(g, stream);
+    else if (fits<NF4, 1, 1, NF4 ? 3 : 4, NF4 ? 24 : 16>(g, g.rows))
+      launch<NF4, 1, 1, NF4 ? 3 : 4, NF4 ? 24 : 16>(g, stream);
     else
-      launch<NF4, 1, 1, 2, 2>(g, stream);
+      launch<NF4, 1, 1, 2, 16>(g, stream);
     rows -= g.rows;
     g.x += size_t(g.rows) * g.in;
     g.y += size_t(g.rows) * cols;
