@@ -22,7 +22,7 @@ using namespace ptx;
 constexpr int kThreads = 512;
 constexpr int kLanes = 16;                  // threads of one head's vector, 8 channels each
 constexpr int kAtOnce = kThreads / kLanes;  // vectors a block works on at once
-constexpr int kQueryHeads = 4;              // query heads a block of the page form rotates
+constexpr int kQueryHeads = 8;              // query heads a block of the page form rotates
 constexpr int kFewTokens = 4;               // new tokens of a sequence up to which a warp takes a (page, head)
 constexpr int kHeld = 2;                    // vectors a thread of the page form holds between its two passes
 
@@ -88,26 +88,36 @@ __device__ __forceinline__ Angles angles_of(const KvCacheView& c, const RotaryAr
   return a;
 }
 
-// Norm (w: the weight's two pieces, or none) and rotation of one head vector spread over 16 lanes, in fp32. Whole warps.
+// Norm (w: the weight's two pieces, or none) and rotation of one head vector spread over 16 lanes, in fp32, two channels an instruction.
+// Whole warps.
 __device__ __forceinline__ void norm_rope(float (&v)[8], bool norm, const float (&w)[8], float eps, bool turns, const Angles& t) {
-  if (norm) {
-    float sum = 0.0f;
+  f32x2 x[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
+  for (int i = 0; i < 4; ++i) x[i] = pack2(v[2 * i], v[2 * i + 1]);
+  if (norm) {
+    f32x2 sum2 = mul2(x[0], x[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) sum2 = fma2(x[i], x[i], sum2);
+    float lo, hi;
+    unpack2(sum2, lo, hi);
+    float sum = lo + hi;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     const float inv = rsqrtf(fmaf(sum, 1.0f / kKvHeadDim, eps));
+    const f32x2 inv2 = pack2(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+    for (int i = 0; i < 4; ++i) x[i] = mul2(mul2(x[i], inv2), pack2(w[2 * i], w[2 * i + 1]));
   }
   if (turns) {
-    const float c[4] = {t.c.x, t.c.y, t.c.z, t.c.w}, s[4] = {t.s.x, t.s.y, t.s.z, t.s.w};
+    const f32x2 c[2] = {pack2(t.c.x, t.c.y), pack2(t.c.z, t.c.w)}, s[2] = {pack2(t.s.x, t.s.y), pack2(t.s.z, t.s.w)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = v[i], b = v[4 + i];
-      v[i] = fmaf(a, c[i], -(b * s[i])), v[4 + i] = fmaf(b, c[i], a * s[i]);
+    for (int i = 0; i < 2; ++i) {
+      const f32x2 a = x[i], b = x[2 + i];
+      x[i] = sub2(mul2(a, c[i]), mul2(b, s[i])), x[2 + i] = fma2(b, c[i], mul2(a, s[i]));
     }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(x[i], v[2 * i], v[2 * i + 1]);
 }
 
 // Codes that are there, rounded again for a larger scale. V has `slots` of each channel's 2^page_shift.
@@ -240,19 +250,29 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView
           const Angles t = angles_of(c, rot, at, run.row0 + i, run.begin + i);
           const __nv_bfloat16* src = g.q + size_t(run.row0 + i) * g.ld_q + head0 * kKvHeadDim;
           __nv_bfloat16* dst = g.q_out + size_t(run.row0 + i) * g.ld_q_out + head0 * kKvHeadDim;
-          uint2 raw[kQueryHeads][2];
+          // two heads at a time, the next two on their way
+          uint2 raw[2][2][2];
+          auto fetch = [&](int h, uint2 (&to)[2][2]) {
 #pragma unroll
-          for (int h = 0; h < kQueryHeads; ++h)
-            if (h < heads) raw[h][0] = load4(src + h * kKvHeadDim + at.a), raw[h][1] = load4(src + h * kKvHeadDim + at.b);
+            for (int k = 0; k < 2; ++k) {
+              const __nv_bfloat16* from = src + min(h + k, heads - 1) * kKvHeadDim;
+              to[k][0] = load4(from + at.a), to[k][1] = load4(from + at.b);
+            }
+          };
+          fetch(0, raw[0]);
 #pragma unroll
-          for (int h = 0; h < kQueryHeads; ++h) {
+          for (int h = 0; h < kQueryHeads; h += 2) {
             if (h >= heads) break;
-            float v[8];
-            widen(raw[h][0], v), widen(raw[h][1], v + 4);
-            norm_rope(v, norm, w, rot.eps, at.turns, t);
-            if (live) {
-              *reinterpret_cast<uint2*>(dst + h * kKvHeadDim + at.a) = narrow(v);
-              *reinterpret_cast<uint2*>(dst + h * kKvHeadDim + at.b) = narrow(v + 4);
+            if (h + 2 < kQueryHeads) fetch(h + 2, raw[(h / 2 + 1) & 1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              float v[8];
+              widen(raw[(h / 2) & 1][k][0], v), widen(raw[(h / 2) & 1][k][1], v + 4);
+              norm_rope(v, norm, w, rot.eps, at.turns, t);
+              if (live && h + k < heads) {
+                *reinterpret_cast<uint2*>(dst + (h + k) * kKvHeadDim + at.a) = narrow(v);
+                *reinterpret_cast<uint2*>(dst + (h + k) * kKvHeadDim + at.b) = narrow(v + 4);
+              }
             }
           }
         }
