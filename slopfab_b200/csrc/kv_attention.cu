@@ -27,7 +27,6 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 64;        // tokens a warp takes at a time
 constexpr int kTileBytes = kTile * kKvHeadDim;  // of K, and of V
 constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
@@ -39,6 +38,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Four e4m3 of a word as two pairs of fp16.
 __device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -86,9 +90,9 @@ __device__ __noinline__ void note_nan(uint32_t* columns, uint32_t bad, int at, i
   }
 }
 
-template <int NT>
-__global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
-  constexpr int kCols = NT * 8;
+template <int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
+  constexpr int kCols = NT * 8, kThreads = kWarps * 32;
   // a tile of K [64 tokens][128] and of V [128][64 tokens] for each warp; when they are done, [kWarps][128][kCols + 1] sums
   extern __shared__ __align__(128) uint8_t smem[];
   float* const sh_o = reinterpret_cast<float*>(smem);
@@ -97,7 +101,6 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
   __shared__ int sh_seen[kWarps][kCols];
   __shared__ uint2 sh_q[8][NT][32];
   __shared__ uint32_t sh_nan[kKvHeadDim];  // columns that are NaN in a channel
-  static_assert(kKvHeadDim == kThreads, "a thread clears a channel");
   __shared__ float sh_qscale[kCols];
   grid_dependency_release();
   grid_dependency_wait();
@@ -113,7 +116,50 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
     const int all_cols = s.rows * g.group;
     for (int col0 = int(blockIdx.x) / splits * kCols; col0 < all_cols; col0 += int(gridDim.x) / splits * kCols) {
       __syncthreads();  // what the tile in front left in shared memory has been read
-      sh_nan[threadIdx.x] = 0;
+      if (threadIdx.x < kKvHeadDim) sh_nan[threadIdx.x] = 0;
+      // ---- this warp's tiles, the first on its way under the queries
+      const int last = min(length, past + min(col0 + kCols - 1, all_cols - 1) / g.group + 1);  // keys that any column sees
+      const int first_hidden = past + col0 / g.group + 1;  // ... that one of them does not
+      const int tiles = (max(last, 0) + kTile - 1) / kTile, per_split = (tiles + splits - 1) / splits;
+      const int tile_end = min(tiles, (split + 1) * per_split);
+      // A tile's pages: lane c holds that of chunk c % 4 of its four chunks of 16 tokens, -1 where there is none.
+      auto page_of = [&](int tile) -> int {
+        const int t = tile * kTile + q * 16;
+        return tile < tile_end && t < last ? kv_page(c, b, t >> c.page_shift) : -1;
+      };
+      const uint32_t k_sh = smem_u32(smem) + warp * 2 * kTileBytes, v_sh = k_sh + kTileBytes;
+      // K: 16 bytes of four tokens at a time, the unit exclusive-or'ed with four times the token's last bit, so that the two rows that eight
+      // lanes read together lie in different banks. V: 16 tokens of eight channels at a time. Chunks without a page are zeros.
+      auto fetch_k = [&](int tile, int pages) {
+        if (tile < tile_end) {
+          const int unit = lane & 7, token0 = lane >> 3;
+          const uint32_t to = k_sh + token0 * 128 + ((unit ^ ((token0 & 1) << 2)) << 4);
+#pragma unroll
+          for (int chunk = 0; chunk < 4; ++chunk) {
+            const int page = __shfl_sync(0xffffffffu, pages, chunk);
+            const int slot = (tile * kTile + chunk * 16) & page_mask;
+            const uint8_t* from = page < 0 ? c.k : c.k + (((size_t(page) * c.kv_heads + head) << c.page_shift) + slot + token0) * kKvHeadDim + unit * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cp_async16(to + (chunk * 16 + i * 4) * 128, from + (page < 0 ? 0 : i * 4 * kKvHeadDim), page < 0 ? 0 : 16);
+          }
+        }
+        cp_commit();
+      };
+      auto fetch_v = [&](int tile, int pages) {
+        if (tile < tile_end) {
+          const int slot = (tile * kTile + q * 16) & page_mask;
+          const uint8_t* from = pages < 0 ? c.v : c.v + (((size_t(pages) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
+          const int step = pages < 0 ? 0 : 8 << c.page_shift;
+          const uint32_t to = v_sh + gq * 64 + q * 16;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) cp_async16(to + i * 8 * 64, from + i * step, pages < 0 ? 0 : 16);
+        }
+        cp_commit();
+      };
+      int tile = split * per_split + warp;
+      int pages = page_of(tile), next_pages = page_of(tile + kWarps);
+      fetch_k(tile, pages);
+      fetch_v(tile, pages);
       // ---- the queries as fp16, each times a power of two that takes its largest element just below 2^15. Its eight significant bits are
       // exact down to 2^-31 of that; what is smaller is off by 2^-39 of it at most.
       for (int i = threadIdx.x; i < kCols * 4; i += kThreads) {
@@ -164,54 +210,12 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
           qscale[n][e] = sh_qscale[col];
           m[n][e] = mv[n][e] = -INFINITY, l[n][e] = 0.0f, seen[n][e] = false;
         }
-      const int last = min(length, past + min(col0 + kCols - 1, all_cols - 1) / g.group + 1);  // keys that any column sees
-      const int first_hidden = past + col0 / g.group + 1;  // ... that one of them does not
-      const int tiles = (max(last, 0) + kTile - 1) / kTile, per_split = (tiles + splits - 1) / splits;
-      const int tile_end = min(tiles, (split + 1) * per_split);
       float o[8][NT][4];
 #pragma unroll
       for (int d = 0; d < 8; ++d)
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[d][n][0] = o[d][n][1] = o[d][n][2] = o[d][n][3] = 0.0f;
 
-      // A tile's pages: lane c holds that of chunk c % 4 of its four chunks of 16 tokens, -1 where there is none.
-      auto page_of = [&](int tile) -> int {
-        const int t = tile * kTile + q * 16;
-        return tile < tile_end && t < last ? kv_page(c, b, t >> c.page_shift) : -1;
-      };
-      const uint32_t k_sh = smem_u32(smem) + warp * 2 * kTileBytes, v_sh = k_sh + kTileBytes;
-      // K: 16 bytes of four tokens at a time, the unit exclusive-or'ed with four times the token's last bit, so that the two rows that eight
-      // lanes read together lie in different banks. V: 16 tokens of eight channels at a time. Chunks without a page are zeros.
-      auto fetch_k = [&](int tile, int pages) {
-        if (tile < tile_end) {
-          const int unit = lane & 7, token0 = lane >> 3;
-          const uint32_t to = k_sh + token0 * 128 + ((unit ^ ((token0 & 1) << 2)) << 4);
-#pragma unroll
-          for (int chunk = 0; chunk < 4; ++chunk) {
-            const int page = __shfl_sync(0xffffffffu, pages, chunk);
-            const int slot = (tile * kTile + chunk * 16) & page_mask;
-            const uint8_t* from = page < 0 ? c.k : c.k + (((size_t(page) * c.kv_heads + head) << c.page_shift) + slot + token0) * kKvHeadDim + unit * 16;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) cp_async16(to + (chunk * 16 + i * 4) * 128, from + (page < 0 ? 0 : i * 4 * kKvHeadDim), page < 0 ? 0 : 16);
-          }
-        }
-        cp_commit();
-      };
-      auto fetch_v = [&](int tile, int pages) {
-        if (tile < tile_end) {
-          const int slot = (tile * kTile + q * 16) & page_mask;
-          const uint8_t* from = pages < 0 ? c.v : c.v + (((size_t(pages) * c.kv_heads + head) * kKvHeadDim + gq) << c.page_shift) + slot;
-          const int step = pages < 0 ? 0 : 8 << c.page_shift;
-          const uint32_t to = v_sh + gq * 64 + q * 16;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) cp_async16(to + i * 8 * 64, from + i * step, pages < 0 ? 0 : 16);
-        }
-        cp_commit();
-      };
-      int tile = split * per_split + warp;
-      int pages = page_of(tile), next_pages = page_of(tile + kWarps);
-      fetch_k(tile, pages);
-      fetch_v(tile, pages);
       for (; tile < tile_end; tile += kWarps) {
         const int t0 = tile * kTile;
         const size_t block = size_t(max(pages, 0)) * c.kv_heads + head;
@@ -221,33 +225,34 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
         __syncwarp();
         float sc[4][NT][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          uint4 k[2][2];  // [row gq or gq + 8][half of the channels]
-          const int token = (gq >> 1) * 16 + t * 4 + (gq & 1);
+        for (int t = 0; t < 4; t += 2) {  // two MMAs of 16 tokens share the reads of q
+          uint4 k[2][2][2];  // [MMA][row gq or gq + 8][half of the channels]
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) k[r][u] = lds128(k_sh + (token + 2 * r) * 128 + (((u * 4 + q) ^ ((gq & 1) << 2)) << 4));
-          float odd[NT][4];
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[t][n][e] = odd[n][e] = 0.0f;
+              for (int u = 0; u < 2; ++u)
+                k[i][r][u] = lds128(k_sh + ((gq >> 1) * 16 + (t + i) * 4 + (gq & 1) + 2 * r) * 128 + (((u * 4 + q) ^ ((gq & 1) << 2)) << 4));
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            uint32_t a0, a1, a2, a3;
-            e4m3_pairs(word_of(k[0][j >> 2], j & 3), a0, a2);
-            e4m3_pairs(word_of(k[1][j >> 2], j & 3), a1, a3);
+            uint2 bq[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint2 bq = sh_q[j][n][lane];
-              mma_f16(j & 1 ? odd[n] : sc[t][n], a0, a1, a2, a3, bq.x, bq.y);
+            for (int n = 0; n < NT; ++n) bq[n] = sh_q[j][n][lane];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a0, a1, a2, a3;
+              e4m3_pairs(word_of(k[i][0][j >> 2], j & 3), a0, a2);
+              e4m3_pairs(word_of(k[i][1][j >> 2], j & 3), a1, a3);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                if (j == 0)
+                  mma_f16_zero(sc[t + i][n], a0, a1, a2, a3, bq[n].x, bq[n].y);
+                else
+                  mma_f16(sc[t + i][n], a0, a1, a2, a3, bq[n].x, bq[n].y);
+              }
             }
           }
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[t][n][e] += odd[n][e];
         }
         __syncwarp();
         fetch_k(tile + kWarps, next_pages);
@@ -314,6 +319,19 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[d][n][e] *= keep[n][e & 1];
         }
+        // Where the references lie near each other, as they do unless pages' scales differ by a great deal, the second weight is the first
+        // times a factor.
+        float factor[NT][2];
+        bool near = true;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float between = m[n][e] == -INFINITY ? 0.0f : m[n][e] - mv[n][e] + e_mine;
+            near &= fabsf(between) < 60.0f;
+            factor[n][e] = exp2_fast(between) * frac;
+          }
+        near = __all_sync(0xffffffffu, near);
         uint32_t p[4][NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -328,8 +346,9 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              l[n][e & 1] += exp2_fast(sc[t][n][e] - ref[e & 1]);
-              w[e] = exp2_fast(sc[t][n][e] + ref_v[e & 1]) * frac;
+              w[e] = exp2_fast(sc[t][n][e] - ref[e & 1]);
+              l[n][e & 1] += w[e];
+              w[e] = near ? w[e] * factor[n][e & 1] : exp2_fast(sc[t][n][e] + ref_v[e & 1]) * frac;
             }
             p[t][n][0] = transpose8x8(half_pair(w[0], w[1]));
             p[t][n][1] = transpose8x8(half_pair(w[2], w[3]));
@@ -451,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, kResident[NT]) kv_attention_kernel(K
 }
 
 // One CTA per row and head: its parts in order, a quarter of them a warp.
-__global__ void __launch_bounds__(kThreads) kv_join_kernel(KvCacheView c, KvAttentionArgs g, const float* parts, int splits) {
+__global__ void __launch_bounds__(128) kv_join_kernel(KvCacheView c, KvAttentionArgs g, const float* parts, int splits) {
+  constexpr int kWarps = 4;
   __shared__ float4 sh_o[kWarps][32];
   __shared__ float sh_l[kWarps];
   grid_dependency_release();
@@ -512,7 +532,7 @@ __global__ void __launch_bounds__(kThreads) kv_join_kernel(KvCacheView c, KvAtte
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 struct AttentionPlan {
-  int nt, col_tiles, splits;
+  int nt, col_tiles, splits, warps;
 };
 
 // How a launch is divided, from the host's estimates.
@@ -523,10 +543,12 @@ AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
   p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
   const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
   const int resident = kResident[p.nt] * kSms;
-  // Few sequences: as many CTAs as run at once. More: twice as many, so that unequal lengths even out. A part of less than 256 tokens
-  // (a tile for each warp) is not worth its joining.
-  const long long want = 4 * ctas <= resident ? resident / ctas : (2 * resident + ctas - 1) / ctas, most = std::max(1, c.max_len / (4 * ctas <= resident ? 256 : 768));
+  // Few sequences: as many CTAs as run at once. More: twice as many, so that unequal lengths even out. A part of less than 512 tokens
+  // is not worth its joining.
+  const long long want = 4 * ctas <= resident ? resident / ctas : (2 * resident + ctas - 1) / ctas, most = std::max(1, c.max_len / (4 * ctas <= resident ? 512 : 768));
   p.splits = int(std::max(1ll, std::min({want, most, (long long)kMostSplits})));
+  // Eight warps a CTA, which is then alone on its SM, where there are no more CTAs than SMs and each has more than a tile for four.
+  p.warps = ctas * p.splits <= kSms && c.max_len > 4 * kTile * p.splits ? 8 : 4;
   return p;
 }
 
@@ -561,13 +583,14 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   const AttentionPlan p = plan_for(c, g.heads, c.rows);
   float* parts = static_cast<float*>(workspace);
   const dim3 grid(p.splits * p.col_tiles, c.kv_heads, std::min(c.batch, 65535));
-  const size_t smem = size_t(kWarps) * 2 * kTileBytes;
-  const auto kernel = p.nt == 1 ? kv_attention_kernel<1> : p.nt == 2 ? kv_attention_kernel<2> : kv_attention_kernel<3>;
+  const size_t smem = size_t(p.warps) * 2 * kTileBytes;
+  const auto kernel = p.warps == 4 ? (p.nt == 1 ? kv_attention_kernel<1, 4> : p.nt == 2 ? kv_attention_kernel<2, 4> : kv_attention_kernel<3, 4>)
+                                   : (p.nt == 1 ? kv_attention_kernel<1, 8> : p.nt == 2 ? kv_attention_kernel<2, 8> : kv_attention_kernel<3, 8>);
   reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "kv attention");
-  cudaError_t e = launch_overlapped(0, kernel, grid, dim3(kThreads), smem, stream, c, g, parts, p.splits);
+  cudaError_t e = launch_overlapped(0, kernel, grid, dim3(p.warps * 32), smem, stream, c, g, parts, p.splits);
   if (e == cudaSuccess && p.splits > 1) {
     const long long units = (long long)std::min(c.max_new, c.rows) * g.heads;
-    e = launch_overlapped(0, kv_join_kernel, dim3(unsigned(std::min(units, 65535ll)), std::min(c.batch, 65535)), dim3(kThreads), 0, stream, c, g,
+    e = launch_overlapped(0, kv_join_kernel, dim3(unsigned(std::min(units, 65535ll)), std::min(c.batch, 65535)), dim3(128), 0, stream, c, g,
                           static_cast<const float*>(parts), p.splits);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("kv attention: launch failed: ") + cudaGetErrorString(e));
