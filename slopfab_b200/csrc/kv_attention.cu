@@ -31,6 +31,7 @@ constexpr int kTile = 64;        // tokens a warp takes at a time
 constexpr int kTileBytes = kTile * kKvHeadDim;  // of K, and of V
 constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
 constexpr int kMostSplits = 64;
+constexpr int kNarrowSplits = 16;  // parts up to which a warp joins them
 constexpr int kSms = 148;        // the launch is planned for; the workspace can be asked for without a device
 constexpr int kResident[4] = {0, 3, 2, 2};  // CTAs of an SM, by the query tiles of eight
 
@@ -469,62 +470,77 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
   }
 }
 
-// One CTA per row and head: its parts in order, a quarter of them a warp.
+// The parts of a row and head in order: a warp for each of them, or (WIDE, many parts) four warps with a quarter of the parts each.
+template <bool WIDE>
 __global__ void __launch_bounds__(128) kv_join_kernel(KvCacheView c, KvAttentionArgs g, const float* parts, int splits) {
-  constexpr int kWarps = 4;
-  __shared__ float4 sh_o[kWarps][32];
-  __shared__ float sh_l[kWarps];
+  constexpr int kWarps = WIDE ? 4 : 1, kEach = WIDE ? kMostSplits / 32 : 1;  // parts a lane looks at
+  static_assert(kNarrowSplits <= 32, "one part a lane");
+  __shared__ float4 sh_o[4][32];
+  __shared__ float sh_l[4];
   grid_dependency_release();
   grid_dependency_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part0 = WIDE ? warp : 0;
   for (int b = blockIdx.y; b < c.batch; b += gridDim.y) {
     const KvSequence s = kv_sequence(c, b);
-    for (long long unit = blockIdx.x; unit < (long long)s.rows * g.heads; unit += gridDim.x) {
-      const int row = s.row0 + int(unit / g.heads), qh = int(unit % g.heads);
+    const int units = s.rows * g.heads;
+    for (int unit = WIDE ? blockIdx.x : blockIdx.x * 4 + warp; unit < units; unit += gridDim.x * (WIDE ? 1 : 4)) {
+      const int row = s.row0 + unit / g.heads, qh = unit % g.heads;
       const float* part = parts + (size_t(row) * g.heads + qh) * splits * kPartFloats;
-      static_assert(kMostSplits == 64, "two parts a lane");
-      float mm = -INFINITY, f[2];
+      float mm = -INFINITY, f[kEach];
       bool any = false;
-      float4 st[2];
+      float4 st[kEach];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kEach; ++h) {
         const int i = lane + 32 * h;
         st[h] = i < splits ? *reinterpret_cast<const float4*>(part + i * kPartFloats + 128) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         mm = fmaxf(mm, st[h].x), any |= st[h].z != 0.0f;
       }
+      const int each = (splits + kWarps - 1) / kWarps, begin = part0 * each, end = min(splits, begin + each);
+      constexpr int kAhead = 4;
+      float4 o[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (begin + k < end) o[k] = *reinterpret_cast<const float4*>(part + (begin + k) * kPartFloats + lane * 4);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
       any = __any_sync(0xffffffffu, any);
       // a part without a finite score has weight 1: it is zeros, or NaN
 #pragma unroll
-      for (int h = 0; h < 2; ++h) f[h] = st[h].x == -INFINITY ? 1.0f : exp2_fast(st[h].x - (mm == -INFINITY ? 0.0f : mm));
+      for (int h = 0; h < kEach; ++h) f[h] = st[h].x == -INFINITY ? 1.0f : exp2_fast(st[h].x - (mm == -INFINITY ? 0.0f : mm));
       float ll = 0.0f;
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const int each = (splits + kWarps - 1) / kWarps, end = min(splits, (warp + 1) * each);
-#pragma unroll 8
-      for (int i = warp * each; i < end; ++i) {
-        const float4 o = *reinterpret_cast<const float4*>(part + i * kPartFloats + lane * 4);
-        const float w = __shfl_sync(0xffffffffu, i < 32 ? f[0] : f[1], i & 31), li = __shfl_sync(0xffffffffu, i < 32 ? st[0].y : st[1].y, i & 31);
-        ll = fmaf(li, w, ll);
-        sum.x = fmaf(o.x, w, sum.x), sum.y = fmaf(o.y, w, sum.y), sum.z = fmaf(o.z, w, sum.z), sum.w = fmaf(o.w, w, sum.w);
+      for (int i0 = begin; i0 < end; i0 += kAhead) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int i = i0 + k;
+          if (i >= end) break;
+          float w = f[0], li = st[0].y;
+#pragma unroll
+          for (int h = 1; h < kEach; ++h) w = i >= 32 * h ? f[h] : w, li = i >= 32 * h ? st[h].y : li;
+          w = __shfl_sync(0xffffffffu, w, i & 31), li = __shfl_sync(0xffffffffu, li, i & 31);
+          ll = fmaf(li, w, ll);
+          sum.x = fmaf(o[k].x, w, sum.x), sum.y = fmaf(o[k].y, w, sum.y), sum.z = fmaf(o[k].z, w, sum.z), sum.w = fmaf(o[k].w, w, sum.w);
+          if (i + kAhead < end) o[k] = *reinterpret_cast<const float4*>(part + (i + kAhead) * kPartFloats + lane * 4);
+        }
       }
-      __syncthreads();  // the row in front has been read
-      sh_o[warp][lane] = sum;
-      if (lane == 0) sh_l[warp] = ll;
-      __syncthreads();
-      if (warp == 0) {
+      if constexpr (WIDE) {
+        __syncthreads();  // the row in front has been read
+        sh_o[warp][lane] = sum;
+        if (lane == 0) sh_l[warp] = ll;
+        __syncthreads();
+        if (warp != 0) continue;
         ll = 0.0f;
         sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 o = sh_o[w][lane];
-          ll += sh_l[w], sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
+          const float4 v = sh_o[w][lane];
+          ll += sh_l[w], sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
-        const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;
-        __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv), hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
-        *reinterpret_cast<uint2*>(g.out + size_t(row) * g.ld_out + qh * kKvHeadDim + lane * 4) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
       }
+      const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * inv, sum.y * inv), hi = __floats2bfloat162_rn(sum.z * inv, sum.w * inv);
+      *reinterpret_cast<uint2*>(g.out + size_t(row) * g.ld_out + qh * kKvHeadDim + lane * 4) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
   }
 }
@@ -570,6 +586,7 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   kv_check(c, head_dim);
   check_heads(c, g.heads);
   if (c.rows <= 0) return;
+  if ((long long)c.rows * g.heads > 0x7FFFFFFF) throw std::invalid_argument("kv attention: too many rows and heads");
   if (!g.q || !g.out) throw std::invalid_argument("kv attention: null operand");
   if (g.ld_q < g.heads * kKvHeadDim || g.ld_out < g.heads * kKvHeadDim || g.ld_q % 8 != 0 || g.ld_out % 8 != 0 || !aligned16(g.q) || !aligned16(g.out))
     throw std::invalid_argument("kv attention: row pitches must cover heads * 128 columns and keep 16-byte alignment");
@@ -589,9 +606,10 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "kv attention");
   cudaError_t e = launch_overlapped(0, kernel, grid, dim3(p.warps * 32), smem, stream, c, g, parts, p.splits);
   if (e == cudaSuccess && p.splits > 1) {
-    const long long units = (long long)std::min(c.max_new, c.rows) * g.heads;
-    e = launch_overlapped(0, kv_join_kernel, dim3(unsigned(std::min(units, 65535ll)), std::min(c.batch, 65535)), dim3(128), 0, stream, c, g,
-                          static_cast<const float*>(parts), p.splits);
+    const bool wide = p.splits > kNarrowSplits;
+    const long long units = (long long)std::min(c.max_new, c.rows) * g.heads, ctas = wide ? units : (units + 3) / 4;
+    e = launch_overlapped(0, wide ? kv_join_kernel<true> : kv_join_kernel<false>, dim3(unsigned(std::min(ctas, 65535ll)), std::min(c.batch, 65535)), dim3(128), 0,
+                          stream, c, g, static_cast<const float*>(parts), p.splits);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("kv attention: launch failed: ") + cudaGetErrorString(e));
 }

@@ -92,7 +92,7 @@ def test_append_refuses_rotations(over):
     assert _append(_cache(), rotary=sfq.RotaryDesc(**f)) == sfq.ERR_INVALID_ARGUMENT
 
 
-@pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(heads=0), dict(heads=3), dict(ld_q=504),
+@pytest.mark.parametrize("over", [dict(rows=1 << 29), dict(q=None), dict(out=None), dict(heads=0), dict(heads=3), dict(ld_q=504),
                                   dict(ld_out=516), dict(out=A), dict(q=A + 8), dict(out=2 * A + 2)])
 def test_attention_refuses_operands(over):
     assert _attend(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
