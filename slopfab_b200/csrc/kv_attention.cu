@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <stdexcept>
 #include <string>
 
@@ -558,13 +559,19 @@ AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
   p.nt = cols > 16 ? 3 : cols > 8 ? 2 : 1;
   p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
   const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
-  const int resident = kResident[p.nt] * kSms;
-  // Few sequences: as many CTAs as run at once. More: twice as many, so that unequal lengths even out. A part of less than 512 tokens
-  // is not worth its joining.
-  const long long want = 4 * ctas <= resident ? resident / ctas : (2 * resident + ctas - 1) / ctas, most = std::max(1, c.max_len / (4 * ctas <= resident ? 512 : 768));
-  p.splits = int(std::max(1ll, std::min({want, most, (long long)kMostSplits})));
-  // Eight warps a CTA, which is then alone on its SM, where there are no more CTAs than SMs and each has more than a tile for four.
-  p.warps = ctas * p.splits <= kSms && c.max_len > 4 * kTile * p.splits ? 8 : 4;
+  // Waves of CTAs times what a CTA takes: about 4 us around its tiles and, with its SM full, 4.5 us for one of a warp's tiles (one query tile
+  // of eight; 6.5 and 10 with two and three), and 2 us for joining. A CTA of eight warps is alone on its SM. 32 sequences of up to 4096
+  // tokens, 8 kv heads: 57.8 / 50.5 / 48.6 / 49.5 / 53.4 us in 1 / 2 / 3 / 4 / 6 parts; one of 131072: 58.6 / 52.8 / 70.7 in 37 / 55 / 64.
+  const int per_tile = p.nt == 1 ? 45 : p.nt == 2 ? 65 : 100, tiles = (c.max_len - 1) / kTile + 1;
+  long long best = LLONG_MAX;
+  for (int warps = 4; warps <= 8; warps += 4) {
+    const long long resident = (warps == 4 ? kResident[p.nt] : 1) * kSms;
+    for (int splits = 1; splits <= std::min(kMostSplits, tiles); ++splits) {
+      const long long waves = (ctas * splits + resident - 1) / resident, each = ((tiles + splits - 1) / splits + warps - 1) / warps;
+      const long long cost = waves * (40 + each * per_tile) + (splits > 1 ? 20 : 0);
+      if (cost < best) best = cost, p.splits = splits, p.warps = warps;
+    }
+  }
   return p;
 }
 
