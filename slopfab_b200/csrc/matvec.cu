@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "codec.cuh"
 #include "kernels.cuh"
@@ -37,9 +38,18 @@ constexpr int kTableBytes = 65536; // NF4: entry of byte b for lane l at b * 256
 // Floats of a row of a warp's sums: one more than it has, against bank conflicts, where there is room.
 __host__ __device__ constexpr int sum_pitch(bool nf4, int nt) { return nt * 8 + (nf4 && nt == 2 ? 0 : 1); }
 
+struct Zero {  // a number that is known to be 0
+  __device__ __forceinline__ Zero(int) {}
+  __device__ __forceinline__ constexpr operator int() const { return 0; }
+};
+
+// What a team's sums of a unit take in a cluster's exchange: at most 256 outputs, halves of SwiGLU pairs counted, and a share that is rounded up.
+constexpr int kSwapBytes = 1024 + 64;
+
 struct Plan {
   int units = 0;  // groups of MT tiles of 16 weight rows
-  int ring_off = 0, part_off = 0, x_off = 0;  // byte offsets into shared memory
+  int ring_off = 0, part_off = 0, swap_off = 0, x_off = 0;  // byte offsets into shared memory
+  int cluster = 1;  // CTAs that divide K
 };
 
 __device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -78,6 +88,8 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
+
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory"); }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -134,7 +146,7 @@ __device__ __forceinline__ float banded(float f, int e, int band) {
   return ldexpf(f, 14 - e + 32 * band);
 }
 
-template <bool NF4, int NT, int MT, int D, int WARPS, int kTeamWarps>
+template <bool NF4, int NT, int MT, int D, int WARPS, int kTeamWarps, bool CLUSTER>
 __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_kernel(MatvecArgs g, Plan p) {
   constexpr int kThreads = WARPS * 32, TEAMS = WARPS / kTeamWarps;
   constexpr int kStage = MT * 1024 + (NF4 ? 0 : MT * 128);  // codes [MT][16 rows][64 bytes], scales [MT][2 slabs][16 rows][4 bytes]
@@ -144,26 +156,31 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
   __shared__ float nested_map[NF4 ? 256 : 1];
   const int warp = (threadIdx.x >> 5) % kTeamWarps, team = threadIdx.x / (kTeamWarps * 32), lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
   const bool swiglu = g.act == SFQ_ACT_SWIGLU;
-  const int steps = (g.in + kStep - 1) / kStep;
+  // A cluster's CTAs take the same rows and each its part of K, steps begin .. end - 1.
+  const int cluster = CLUSTER ? p.cluster : 1, rank = CLUSTER ? int(cluster_ctarank()) : 0;
+  const int first_cta = CLUSTER ? int(blockIdx.x) / cluster : int(blockIdx.x), all_ctas = CLUSTER ? int(gridDim.x) / cluster : int(gridDim.x);
+  const int all_steps = (g.in + kStep - 1) / kStep, steps = CLUSTER ? all_steps * (rank + 1) / cluster : all_steps;
+  const std::conditional_t<CLUSTER, int, Zero> begin = all_steps * rank / cluster;
   const uint32_t base = smem_u32(smem);
   const uint32_t ring = base + p.ring_off + (threadIdx.x >> 5) * D * kStage;
-  const int first_unit = team * gridDim.x + blockIdx.x, all_teams = gridDim.x * TEAMS;  // what is left over falls on different CTAs
+  const int first_unit = team * all_ctas + first_cta, all_teams = all_ctas * TEAMS;  // what is left over falls on different CTAs
   grid_dependency_release();
+  if constexpr (CLUSTER) cluster_arrive();  // this CTA's shared memory is there
 
   // The copies under way: the next one is step `fs` of unit `fu`.
   int fu, fs;
   const uint8_t* src[MT][2];     // this lane's 16 bytes of rows gq and gq + 8 of each tile
   const uint8_t* scale_src[MT];  // NVFP4: four scales of row lane % 16, slab lane / 16
   auto seek = [&](int unit) {
-    fu = unit, fs = warp;
+    fu = unit, fs = int(begin) + warp;
     if (unit >= p.units) return;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        src[m][h] = g.data + size_t(weight_row<NF4>(unit * MT + m, gq + 8 * h, g.out, swiglu)) * (g.in / 2) + q * 16 + size_t(warp) * (kStep / 2);
+        src[m][h] = g.data + size_t(weight_row<NF4>(unit * MT + m, gq + 8 * h, g.out, swiglu)) * (g.in / 2) + q * 16 + size_t(int(begin) + warp) * (kStep / 2);
       if constexpr (!NF4)
-        scale_src[m] = g.scale + nvfp4_scale_offset(weight_row<NF4>(unit * MT + m, lane & 15, g.out, swiglu), (lane >> 4) * 4, g.in / 16) + size_t(warp) * (kStep * 8);
+        scale_src[m] = g.scale + nvfp4_scale_offset(weight_row<NF4>(unit * MT + m, lane & 15, g.out, swiglu), (lane >> 4) * 4, g.in / 16) + size_t(int(begin) + warp) * (kStep * 8);
     }
   };
   const uint32_t code_at = gq * 64 + (NF4 ? q ^ (gq & 2) : q) * 16;  // in a tile's codes; NF4 is read in 8-byte pieces of four rows at a time
@@ -228,7 +245,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
   // x [rows, in] as fp16: 16 bytes of eight elements, pairs with the odd element in the low half, at unit
   // ((step * 4 + piece) * rows + row) * 4 + lane % 4, which is the order in which the MMAs' lanes read them.
   auto stage_x = [&](int band) -> bool {  // band < 0: the first attempt; true where an element does not fit it
-    const int units = steps * kStep / 8;
+    const int units = (steps - int(begin)) * kStep / 8, k0 = int(begin) * kStep;
     const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x3400), __ushort_as_bfloat16(0x3400));  // 2^-23
     const __nv_bfloat162 sixty_four = __halves2bfloat162(__ushort_as_bfloat16(0x4280), __ushort_as_bfloat16(0x4280));
     const __nv_bfloat162 zero = __halves2bfloat162(__ushort_as_bfloat16(0), __ushort_as_bfloat16(0));
@@ -236,6 +253,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
     __nv_bfloat162 top = zero;
     constexpr int kBatch = (!NF4 && D == 4) || WARPS > 16 ? 4 : 8;  // loads in flight
     int r = 0, k8 = threadIdx.x;
+    if (CLUSTER && units == 0) return false;
     while (k8 >= units) k8 -= units, ++r;
     while (r < g.rows) {
       uint4 raw[kBatch];
@@ -243,7 +261,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         rr[i] = r, kk[i] = k8;
-        raw[i] = r < g.rows && k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(g.x + size_t(r) * g.in + k8 * 8) : make_uint4(0, 0, 0, 0);
+        raw[i] = r < g.rows && k0 + k8 * 8 < g.in ? *reinterpret_cast<const uint4*>(g.x + size_t(r) * g.in + k0 + k8 * 8) : make_uint4(0, 0, 0, 0);
         k8 += kThreads;
         while (k8 >= units) k8 -= units, ++r;
       }
@@ -281,7 +299,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
   for (int n = 0; n < NT; ++n) x_at[n] = base + p.x_off + (min(gq + 8 * n, g.rows - 1) * 4 + q) * 16;
   const uint32_t x_piece = g.rows * 64;
   auto multiply = [&](int s, uint32_t from) {
-    const uint32_t xs = s * 4 * x_piece;
+    const uint32_t xs = (s - int(begin)) * 4 * x_piece;
     if constexpr (!NF4) {
       uint4 w[MT][2];
       uint32_t sc[MT][2];
@@ -363,7 +381,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
   // This warp's steps of a unit. Their first D - 1 copies are under way, and go on with the units up to end_unit.
   uint32_t slot = 0;  // byte offset into the ring
   auto walk = [&](int unit, int end_unit) {
-    for (int s = warp; s < steps; s += kTeamWarps) {
+    for (int s = int(begin) + warp; s < steps; s += kTeamWarps) {
       cp_wait<D - 2>();
       __syncwarp();  // the copies have landed in every lane, and the step in front has been read
       fetch(ring + (slot == 0 ? (D - 1) * kStage : slot - kStage), end_unit);
@@ -374,7 +392,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
           fetch_absmax(s + kTeamWarps);
         } else if (unit + all_teams < end_unit) {
           seek_absmax(unit + all_teams);
-          fetch_absmax(warp);
+          fetch_absmax(int(begin) + warp);
         }
       }
       multiply(s, ring + slot);
@@ -386,22 +404,25 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
     __syncwarp();
     seek(unit);
     for (int i = 0; i < D - 1; ++i) fetch(ring + i * kStage, end_unit);
-    if (unit < end_unit && warp < steps) {
+    if (unit < end_unit && int(begin) + warp < steps) {
       seek_absmax(unit);
-      fetch_absmax(warp);
+      fetch_absmax(int(begin) + warp);
     }
   };
 
-  // The team's sums of a unit, added in the order of its warps, finished and stored.
-  // NF4 keeps them in the unused halves of the table's lines.
+  // The team's sums of a unit, added in the order of its warps, finished and stored. NF4 keeps them in the unused halves of the table's
+  // lines. In a cluster each CTA finishes its share of the outputs: the others' shares go to them, over the row's power of two and the
+  // tensor scale, and are added in the order of the ranks. Every team of every CTA takes part for every unit (those without one as -1),
+  // and the two buffers take turns, so that one barrier a unit is enough.
   const int part0 = team * kTeamWarps * MT * 16 * kPitch;
   auto part = [&](int i) -> float& {
     const int at = part0 + i;
     return *reinterpret_cast<float*>(smem + (NF4 ? (at >> 5) * 256 + 128 + (at & 31) * 4 : p.part_off + at * 4));
   };
-  const int cols = swiglu ? g.out / 2 : g.out;
-  auto finish = [&](int unit) {
-    named_barrier(team + 1, kTeamWarps * 32);  // the sums of the unit in front have been read
+  const int cols = swiglu ? g.out / 2 : g.out, per_tile = swiglu ? 8 : 16, halves = swiglu ? 2 : 1;
+  const int outputs = MT * per_tile * g.rows, share = (outputs + cluster - 1) / cluster;
+  auto gather = [&](int unit) {  // every warp's sums into shared memory
+    named_barrier(team + 1, kTeamWarps * 32);  // those of the unit in front have been read
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -409,21 +430,52 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
 #pragma unroll
         for (int e = 0; e < 4; ++e) part((warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)) = acc[m][n][e];
     named_barrier(team + 1, kTeamWarps * 32);
-    const int per_tile = swiglu ? 8 : 16;
-    for (int i = warp * 32 + lane; i < MT * per_tile * g.rows; i += kTeamWarps * 32) {
-      const int r = i / (MT * per_tile), local = i - r * (MT * per_tile), m = local / per_tile, j = local - m * per_tile;
-      const int n = weight_row<NF4>(unit * MT + m, j, g.out, swiglu);
-      if (NF4 && (unit * MT + m) * per_tile + j >= cols) continue;
-      float z[2] = {0.0f, 0.0f};
-      for (int h = 0; h < (swiglu ? 2 : 1); ++h) {
-        float s = 0.0f;
+  };
+  auto summed = [&](int r, int row) {  // the team's sum of a row of the tiles and a row of x
+    float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kTeamWarps; ++w) s += part((w * MT * 16 + m * 16 + j + 8 * h) * kPitch + r);
-        const int at = n + h * cols;
-        const float b = g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
-        z[h] = ldexpf(s * g.global_scale, row_e[r] - 14) + b;
+    for (int w = 0; w < kTeamWarps; ++w) s += part((w * MT * 16 + row) * kPitch + r);
+    return ldexpf(s * g.global_scale, row_e[r] - 14);
+  };
+  auto bias_of = [&](int at) {
+    return g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
+  };
+  int turn = 0;
+  auto finish = [&](int unit) {
+    const uint32_t swap = base + p.swap_off + turn * TEAMS * kSwapBytes + team * kSwapBytes;  // cluster: [rank][halves][share]
+    if (unit >= 0) {
+      gather(unit);
+      for (int i = warp * 32 + lane; i < outputs; i += kTeamWarps * 32) {
+        const int r = i / (MT * per_tile), local = i - r * (MT * per_tile), m = local / per_tile, j = local - m * per_tile;
+        if constexpr (!CLUSTER) {
+          const int n = weight_row<NF4>(unit * MT + m, j, g.out, swiglu);
+          if (NF4 && (unit * MT + m) * per_tile + j >= cols) continue;
+          float z[2] = {0.0f, 0.0f};
+          for (int h = 0; h < (swiglu ? 2 : 1); ++h) z[h] = summed(r, m * 16 + j + 8 * h) + bias_of(n + h * cols);
+          g.y[size_t(r) * cols + n] = __float2bfloat16(activated(z[0], z[1], g.act));
+        } else {
+          const int owner = i / share;
+          for (int h = 0; h < halves; ++h)
+            st_cluster(map_to_rank(swap + ((rank * halves + h) * share + i - owner * share) * 4, owner), summed(r, m * 16 + j + 8 * h));
+        }
       }
-      g.y[size_t(r) * cols + n] = __float2bfloat16(activated(z[0], z[1], g.act));
+    }
+    if constexpr (CLUSTER) {
+      cluster_sync_all();
+      if (unit >= 0) {
+        for (int i = rank * share + warp * 32 + lane; i < min(outputs, (rank + 1) * share); i += kTeamWarps * 32) {
+          const int r = i / (MT * per_tile), local = i - r * (MT * per_tile), m = local / per_tile, j = local - m * per_tile;
+          const int n = weight_row<NF4>(unit * MT + m, j, g.out, swiglu);
+          if (NF4 && (unit * MT + m) * per_tile + j >= cols) continue;
+          float z[2] = {0.0f, 0.0f};
+          for (int h = 0; h < halves; ++h) {
+            for (int k = 0; k < cluster; ++k) z[h] += __uint_as_float(lds32(swap + ((k * halves + h) * share + i - rank * share) * 4));
+            z[h] += bias_of(n + h * cols);
+          }
+          g.y[size_t(r) * cols + n] = __float2bfloat16(activated(z[0], z[1], g.act));
+        }
+      }
+      turn ^= 1;
     }
   };
 
@@ -447,7 +499,7 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
     // Each row's largest exponent and lowest band, over its finite elements that are not zero.
     for (int r = threadIdx.x >> 5; r < g.rows; r += kThreads / 32) {
       int most = -1000, least = 1000;
-      for (int k = lane; k < g.in; k += 32) {
+      for (int k = int(begin) * kStep + lane; k < min(steps * kStep, g.in); k += 32) {
         const uint32_t u = __float_as_uint(__bfloat162float(g.x[size_t(r) * g.in + k])) & 0x7FFFFFFFu;
         if (u == 0 || u >= 0x7F800000u) continue;
         const int e = u >= 0x800000u ? int(u >> 23) - 127 : 31 - __clz(int(u)) - 149;
@@ -463,26 +515,46 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
       __syncthreads();
     }
   }
-  if (bands == 0) {
-    for (int unit = first_unit; unit < p.units; unit += all_teams) {
-      scale_sums(0.0f);
-      walk(unit, p.units);
-      finish(unit);
+  if constexpr (CLUSTER) cluster_wait();
+  if constexpr (!CLUSTER) {
+    if (bands == 0) {
+      for (int unit = first_unit; unit < p.units; unit += all_teams) {
+        scale_sums(0.0f);
+        walk(unit, p.units);
+        finish(unit);
+      }
+    } else {
+      for (int first = first_cta; first < p.units; first += all_teams) {  // the teams in step, since x changes under them
+        const int unit = first + team * all_ctas;
+        scale_sums(0.0f);
+        for (int band = bands; band >= 0; --band) {
+          cp_wait<0>();
+          __syncthreads();
+          stage_x(band);
+          __syncthreads();
+          start(unit, min(unit + 1, p.units));
+          if (band < bands) scale_sums(0x1p-32f);
+          if (unit < p.units) walk(unit, unit + 1);
+        }
+        if (unit < p.units) finish(unit);
+      }
     }
   } else {
-    for (int first = blockIdx.x; first < p.units; first += all_teams) {  // the teams in step, since x changes under them
-      const int unit = first + team * gridDim.x;
+    for (int first = first_cta; first < p.units; first += all_teams) {  // all teams of all CTAs in step
+      const int unit = first + team * all_ctas;
       scale_sums(0.0f);
       for (int band = bands; band >= 0; --band) {
-        cp_wait<0>();
-        __syncthreads();
-        stage_x(band);
-        __syncthreads();
-        start(unit, min(unit + 1, p.units));
-        if (band < bands) scale_sums(0x1p-32f);
-        if (unit < p.units) walk(unit, unit + 1);
+        if (bands > 0) {
+          cp_wait<0>();
+          __syncthreads();
+          stage_x(band);
+          __syncthreads();
+          start(unit, min(unit + 1, p.units));
+          if (band < bands) scale_sums(0x1p-32f);
+        }
+        if (unit < p.units) walk(unit, bands > 0 ? unit + 1 : p.units);
       }
-      if (unit < p.units) finish(unit);
+      finish(unit < p.units ? unit : -1);
     }
   }
   cp_wait<0>();
@@ -496,74 +568,131 @@ int log2_of(int v) {
 bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// What a launch with this kernel takes of shared memory for `rows` rows of x.
-template <bool NF4, int NT, int MT, int D, int WARPS> size_t plan(const MatvecArgs& g, int rows, Plan& p) {
+// What a launch with this kernel takes of shared memory for `rows` rows of x, with K divided over `cluster` CTAs.
+template <bool NF4, int NT, int MT, int D, int WARPS> size_t plan(const MatvecArgs& g, int rows, int cluster, Plan& p) {
   const bool swiglu = g.act == SFQ_ACT_SWIGLU;
   const int tiles = NF4 ? ((swiglu ? g.out / 2 : g.out) + (swiglu ? 7 : 15)) / (swiglu ? 8 : 16) : g.out / 16;
   p.units = (tiles + MT - 1) / MT;
+  p.cluster = cluster;
   size_t at = NF4 ? kTableBytes : 0;
   p.ring_off = int(at);
   at += size_t(WARPS) * D * (MT * 1024 + (NF4 ? 0 : MT * 128));
   p.part_off = int(at);
   const size_t sums = size_t(WARPS) * MT * 16 * sum_pitch(NF4, NT) * 4;
-  if (!NF4)
-    at += sums;
-  else if (sums > kTableBytes / 2)
-    return ~size_t(0);
+  if (!NF4) at += sums;
+  static_assert(!NF4 || WARPS * MT * 16 * sum_pitch(NF4, NT) * 4 <= kTableBytes / 2, "the sums lie in the table's gaps");
+  p.swap_off = int(at);
+  if (cluster > 1) at += 2 * (WARPS / 4) * kSwapBytes;
   p.x_off = int(at);
-  return at + size_t((g.in + kStep - 1) / kStep * kStep) * rows * 2;
+  const int steps = (g.in + kStep - 1) / kStep;
+  return at + size_t((steps + cluster - 1) / cluster) * kStep * rows * 2;
 }
 
-template <bool NF4, int NT, int MT, int D, int WARPS> bool fits(const MatvecArgs& g, int rows) {
+template <bool NF4, int NT, int MT, int D, int WARPS> bool fits(const MatvecArgs& g, int rows, int cluster) {
   Plan p;
-  return plan<NF4, NT, MT, D, WARPS>(g, rows, p) <= kMostSmem;
+  return plan<NF4, NT, MT, D, WARPS>(g, rows, cluster, p) <= kMostSmem;
 }
 
-template <bool NF4, int NT, int MT, int D, int WARPS, int TEAM> void launch_team(const MatvecArgs& g, const Plan& p, size_t bytes, int resident, cudaStream_t stream) {
-  reserve_dynamic_smem(reinterpret_cast<const void*>(&matvec_kernel<NF4, NT, MT, D, WARPS, TEAM>), bytes, "matvec");
-  const int ctas = std::min(p.units, resident * device_sm_count());
-  const cudaError_t e = launch_overlapped(size_t(g.out) * g.in / 2, matvec_kernel<NF4, NT, MT, D, WARPS, TEAM>, dim3(ctas), dim3(WARPS * 32), bytes, stream, g, p);
+template <bool NF4, int NT, int MT, int D, int WARPS, int TEAM, bool CLUSTER> void launch_team(const MatvecArgs& g, const Plan& p, size_t bytes, int resident, cudaStream_t stream) {
+  const auto kernel = matvec_kernel<NF4, NT, MT, D, WARPS, TEAM, CLUSTER>;
+  reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, "matvec");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(std::min(p.units, resident * device_sm_count() / p.cluster) * p.cluster);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (p.cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = p.cluster, attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (size_t(g.out) * g.in / 2 <= kOverlapBytes) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr, cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, g, p);
   if (e != cudaSuccess) throw std::runtime_error(std::string("matvec: launch failed: ") + cudaGetErrorString(e));
+}
+
+// Whether the device runs clusters of four such CTAs, with all of an SM's shared memory each.
+bool clusters_run() {
+  static PerDevice<bool> cache;
+  return cache.get([] {
+    const auto kernel = matvec_kernel<true, 2, 1, 2, 16, 8, true>;
+    reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), kMostSmem, "matvec");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(4), cfg.blockDim = dim3(512), cfg.dynamicSmemBytes = kMostSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 4, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    return n >= 16;
+  });
 }
 
 // Teams of eight warps, or of four where that takes no more steps: a warp then walks longer rows of steps and fewer sums are joined.
 // 1 x 5120 -> 15360 NVFP4 13.4 us with eight, 12.1 with four; NF4 3 x 13824 -> 5120, where eight take half the steps, 21.4 against 24.4.
-template <bool NF4, int NT, int MT, int D, int WARPS> void launch(const MatvecArgs& g, cudaStream_t stream) {
+template <bool NF4, int NT, int MT, int D, int WARPS, bool CLUSTER = false> void launch(const MatvecArgs& g, int cluster, cudaStream_t stream) {
   Plan p;
-  const size_t bytes = plan<NF4, NT, MT, D, WARPS>(g, g.rows, p);
+  const size_t bytes = plan<NF4, NT, MT, D, WARPS>(g, g.rows, cluster, p);
   const int resident = !NF4 && D == 4 && bytes <= kMostSmem / 2 - 1024 ? 2 : 1;
-  const int steps = (g.in + kStep - 1) / kStep, sms = resident * device_sm_count();
+  const int steps = ((g.in + kStep - 1) / kStep + cluster - 1) / cluster, ctas = resident * device_sm_count() / cluster;
   auto cost = [&](int team) {
-    const int teams = WARPS / team * sms;
+    const int teams = WARPS / team * ctas;
     return ((p.units + teams - 1) / teams) * ((steps + team - 1) / team);
   };
   if (cost(4) <= cost(8))
-    launch_team<NF4, NT, MT, D, WARPS, 4>(g, p, bytes, resident, stream);
+    launch_team<NF4, NT, MT, D, WARPS, 4, CLUSTER>(g, p, bytes, resident, stream);
   else
-    launch_team<NF4, NT, MT, D, WARPS, 8>(g, p, bytes, resident, stream);
+    launch_team<NF4, NT, MT, D, WARPS, 8, CLUSTER>(g, p, bytes, resident, stream);
+}
+
+// The most rows of x, up to `rows`, that one launch takes.
+template <bool NF4> int most_rows(const MatvecArgs& g, int rows, int cluster) {
+  int most = std::min(rows, kMostRows);
+  while (most > 0 && !(most > 8 ? fits<NF4, 2, 1, 2, 16>(g, most, cluster) : fits<NF4, 1, 1, 2, 16>(g, most, cluster))) --most;
+  return most;
 }
 
 template <bool NF4> void launch_rows(MatvecArgs g, int cols, cudaStream_t stream) {
-  if (!fits<NF4, 1, 1, 2, 16>(g, 1)) throw std::invalid_argument("matvec: in_features too large");
-  int rows = g.rows;
-  while (rows > 0) {
-    // as many rows at a time as x fits into shared memory for, in equal parts
-    int most = std::min(rows, kMostRows);
-    while (most > 1 && !(most > 8 ? fits<NF4, 2, 1, 2, 16>(g, most) : fits<NF4, 1, 1, 2, 16>(g, most))) --most;
-    const int parts = (rows + most - 1) / most;
+  // Where x is too large for the shared memory of one CTA, it goes through in several launches, each of which reads the weight, or K is
+  // divided over clusters of two CTAs, or of four where the weight has few rows. A cluster's CTAs meet for every 16 rows of W, which costs
+  // about a microsecond: NF4 16 x 5120 -> 13824 33.7 us in two launches, 27.7 in clusters of two; 10 x 13376 -> 648 37.0 in three launches,
+  // 17.2 in clusters of four.
+  int rows = g.rows, cluster = 1, most = most_rows<NF4>(g, rows, 1);
+  const int wanted = std::min(rows, kMostRows);
+  for (int c = 2; most < wanted && c <= (g.out / 16 <= device_sm_count() || most == 0 ? 4 : 2) && clusters_run(); c *= 2) {
+    const int with = most_rows<NF4>(g, rows, c);
+    if (most == 0 || (with > 0 && (rows + with - 1) / with < (rows + most - 1) / most)) cluster = c, most = with;
+  }
+  if (most == 0) throw std::invalid_argument("matvec: in_features too large");
+  for (int parts = (rows + most - 1) / most; rows > 0; --parts) {
     g.rows = (rows + parts - 1) / parts;
     // Two tiles a step share the reads of x. NVFP4 needs them from three rows of x on and has two CTAs an SM below that; NF4, bound by its
-    // table's lookups, is better off with 24 warps up to four rows (3 x 13824 -> 5120 21.4 us; 16 warps 26.3; with two tiles, 16 rows
-    // 5120 -> 13824 35.0 against 37.5).
+    // table's lookups, is better off with 24 warps up to four rows (3 x 13824 -> 5120 21.4 us; 16 warps 26.3; with two tiles, 8 rows
+    // 5120 -> 13824 17.5 against 18.8).
     constexpr int kTwoTiles = NF4 ? 2 : 3;  // ring stages
-    if (g.rows > 8)
-      launch<NF4, 2, 1, 2, 16>(g, stream);
-    else if (g.rows > (NF4 ? 4 : 2) && fits<NF4, 1, 2, kTwoTiles, 16>(g, g.rows) && g.out >= 64 * device_sm_count())
-      launch<NF4, 1, 2, kTwoTiles, 16>(g, stream);
-    else if (fits<NF4, 1, 1, NF4 ? 3 : 4, NF4 ? 24 : 16>(g, g.rows))
-      launch<NF4, 1, 1, NF4 ? 3 : 4, NF4 ? 24 : 16>(g, stream);
+    if (cluster > 1 && g.rows > 8)
+      launch<NF4, 2, 1, 2, 16, true>(g, cluster, stream);
+    else if (cluster > 1)
+      launch<NF4, 1, 1, 2, 16, true>(g, cluster, stream);
+    else if (g.rows > 8)
+      launch<NF4, 2, 1, 2, 16>(g, 1, stream);
+    else if (g.rows > (NF4 ? 4 : 2) && fits<NF4, 1, 2, kTwoTiles, 16>(g, g.rows, 1) && g.out >= 64 * device_sm_count())
+      launch<NF4, 1, 2, kTwoTiles, 16>(g, 1, stream);
+    else if (fits<NF4, 1, 1, NF4 ? 3 : 4, NF4 ? 24 : 16>(g, g.rows, 1))
+      launch<NF4, 1, 1, NF4 ? 3 : 4, NF4 ? 24 : 16>(g, 1, stream);
     else
-      launch<NF4, 1, 1, 2, 16>(g, stream);
+      launch<NF4, 1, 1, 2, 16>(g, 1, stream);
     rows -= g.rows;
     g.x += size_t(g.rows) * g.in;
     g.y += size_t(g.rows) * cols;
