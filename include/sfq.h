@@ -462,7 +462,7 @@ SFQ_API int sfq_attention_forward(const void* d_q_bf16, int ld_q, const void* d_
 /* y[rows, out] = act(x[rows, in] W^T + b) for few rows, without a dense copy of the weight and with bf16 activations: W is what the
  * stored bytes say (code x group scale x tensor scale, not rounded to bf16), sums are fp32, the result is rounded once. Formats: SFQ_NVFP4
  * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 64 == 0, block sizes powers of two, of 64 elements at least; the 16
- * table entries are rounded to fp16); no AWQ pre-scale, no ConvRot.
+ * table entries are rounded to fp16); no AWQ pre-scale, no ConvRot; in up to 200000.
  * activation: sfq_activation; SFQ_ACT_SWIGLU takes [gate | up] rows (any even out) and writes out / 2 columns. Any number of rows; the
  * weight is read once for 16 of them. x and the weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
 SFQ_API int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, int rows, int activation, void* d_y_bf16, void* stream);
@@ -508,15 +508,15 @@ typedef struct sfq_rotary {
 } sfq_rotary;
 
 /* Puts the new tokens' k and v [rows, kv_heads * 128] into their pages and writes q [rows, heads * 128] normed and rotated to d_q_out
- * (may be d_q itself; heads 0: no q). The scale of a (page, head) is the smallest power of two s (2^-100 at least) with |x| <= 448 s over
+ * (d_q itself with its pitch, or apart from q, k and v; heads 0: no q). The scale of a (page, head) is the smallest power of two s (2^-100 at least) with |x| <= 448 s over
  * the finite values put there so far; a first token in a page starts it anew, a later one can only raise it, and the codes that are there
  * are then rounded again. Infinities are stored as +-448 s, NaN as NaN. `rotary` may be null. A page that is being written
- * belongs to one sequence. */
+ * belongs to one sequence and stands once in its row of the table. */
 SFQ_API int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rotary, const void* d_q_bf16, int ld_q, void* d_q_out_bf16,
                                 int ld_q_out, int heads, const void* d_k_bf16, const void* d_v_bf16, int ld_kv, int rows, void* stream);
 
 /* out[rows, heads * 128] = softmax(q K^T scale) V over the cache: the i-th of a sequence's n new tokens sees its first length - n + i + 1
- * keys; query head h reads kv head h / (heads / kv_heads). scale <= 0 selects 1 / sqrt(128). A row that sees no key is zero; a NaN or +inf
+ * keys; query head h reads kv head h / (heads / kv_heads). scale <= 0 selects 1 / sqrt(128). out and q lie apart. A row that sees no key is zero; a NaN or +inf
  * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Slots behind a sequence's length may hold
  * anything. The workspace is scratch of one call and needs no initialisation; it may be null where
  * sfq_kv_cache_attention_workspace_bytes gives 0. */

@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
@@ -581,12 +582,13 @@ static void check_heads(const KvCacheView& c, int heads) {
   if (heads <= 0 || heads > 32768 || heads % c.kv_heads != 0) throw std::invalid_argument("kv attention: heads must be a multiple of kv_heads");
 }
 
+static size_t workspace_of(const AttentionPlan& p, int heads, int rows) { return p.splits > 1 ? size_t(rows) * heads * p.splits * kPartFloats * sizeof(float) : 0; }
+
 size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads, int rows) {
   kv_check(c, head_dim);
   check_heads(c, heads);
   if (rows <= 0) return 0;
-  const AttentionPlan p = plan_for(c, heads, rows);
-  return p.splits > 1 ? size_t(rows) * heads * p.splits * kPartFloats * sizeof(float) : 0;
+  return workspace_of(plan_for(c, heads, rows), heads, rows);
 }
 
 void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
@@ -597,14 +599,15 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   if (!g.q || !g.out) throw std::invalid_argument("kv attention: null operand");
   if (g.ld_q < g.heads * kKvHeadDim || g.ld_out < g.heads * kKvHeadDim || g.ld_q % 8 != 0 || g.ld_out % 8 != 0 || !aligned16(g.q) || !aligned16(g.out))
     throw std::invalid_argument("kv attention: row pitches must cover heads * 128 columns and keep 16-byte alignment");
-  if (g.q == g.out) throw std::invalid_argument("kv attention: out may not alias q");
-  const size_t need = kv_attention_workspace_bytes(c, head_dim, g.heads, c.rows);
+  if (rows_overlap(g.q, g.ld_q, g.heads * kKvHeadDim, g.out, g.ld_out, g.heads * kKvHeadDim, c.rows)) throw std::invalid_argument("kv attention: out may not overlap q");
+  if (!std::isfinite(scale)) throw std::invalid_argument("kv attention: scale is not finite");
+  const AttentionPlan p = plan_for(c, g.heads, c.rows);
+  const size_t need = workspace_of(p, g.heads, c.rows);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
     throw std::invalid_argument("kv attention: workspace too small or not 16-byte aligned");
   g.group = g.heads / c.kv_heads;
   g.scale_log2 = (scale > 0.0f ? scale : 0.08838834764831845f) * 1.4426950408889634f;
   c.status = device_status_word();
-  const AttentionPlan p = plan_for(c, g.heads, c.rows);
   float* parts = static_cast<float*>(workspace);
   const dim3 grid(p.splits * p.col_tiles, c.kv_heads, std::min(c.batch, 65535));
   const size_t smem = size_t(p.warps) * 2 * kTileBytes;

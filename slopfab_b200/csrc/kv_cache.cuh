@@ -44,4 +44,14 @@ __device__ __forceinline__ int kv_page(const KvCacheView& c, int b, long long p)
   return page;
 }
 
+// Whether a [rows, cols_a] and b [rows, cols_b] bf16, row pitches ld_a and ld_b, share elements. With different pitches the whole extents
+// are compared.
+inline bool rows_overlap(const void* a, long long ld_a, int cols_a, const void* b, long long ld_b, int cols_b, int rows) {
+  const long long from = static_cast<const char*>(b) - static_cast<const char*>(a), end_a = ((rows - 1) * ld_a + cols_a) * 2, end_b = ((rows - 1) * ld_b + cols_b) * 2;
+  if (from >= end_a || from + end_b <= 0) return false;
+  if (rows == 1 || ld_a != ld_b) return true;
+  const long long pitch = ld_a * 2, apart = (from % pitch + pitch) % pitch;
+  return apart < cols_a * 2ll || apart + cols_b * 2ll > pitch;
+}
+
 }  // namespace sfq

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -10,6 +11,8 @@ from . import KvCacheDesc, RotaryDesc, check, lib, ptr
 from .linear import on_device, raw_stream
 
 HEAD_DIM = 128
+_INT = torch.int32
+_FIELDS = struct.Struct("4P4i3P4i")  # sfq_kv_cache; packed at once, which takes a quarter of the time of ctypes' constructor
 
 
 @dataclass
@@ -22,12 +25,8 @@ class Sequences:
     max_new: int
     max_len: int
 
-    def __setattr__(self, name, value):
-        object.__setattr__(self, "_checked", None)  # what was found about the fields so far
-        object.__setattr__(self, name, value)
 
-
-@dataclass
+@dataclass(frozen=True)
 class Rotary:
     """What happens to q and k on the way into the cache: head norm (bf16 [128] weights) and rotation (fp32 [table_rows, rotary_dim / 2]
     tables) at `position` int32 [rows], or at each token's place in its sequence."""
@@ -48,8 +47,12 @@ class Rotary:
         for t in (self.q_norm, self.k_norm):
             if t is not None and t.shape != (HEAD_DIM,):
                 raise ValueError("norm weights have 128 elements")
+        devices = {t.get_device() for t in (self.cos, self.sin, self.position, self.q_norm, self.k_norm) if t is not None}
+        if len(devices) > 1:
+            raise ValueError("the tables, positions and norm weights lie on one device")
         rows, half = self.cos.shape if self.cos is not None else (0, 0)
-        self.desc = RotaryDesc(ptr(self.cos), ptr(self.sin), ptr(self.position), rows, 2 * half, ptr(self.q_norm), ptr(self.k_norm), self.eps)
+        object.__setattr__(self, "device", devices.pop() if devices else None)
+        object.__setattr__(self, "desc", RotaryDesc(ptr(self.cos), ptr(self.sin), ptr(self.position), rows, 2 * half, ptr(self.q_norm), ptr(self.k_norm), self.eps))
 
 
 class KvCache:
@@ -77,19 +80,14 @@ class KvCache:
 
     def _desc(self, s: Sequences) -> KvCacheDesc:
         t, n, r = s.page_table, s.seq_len, s.row_start
-        at = (self._pool, t.data_ptr(), n.data_ptr(), r.data_ptr())
-        if s._checked is not None and s._checked[0] == at:
-            return s._checked[1]
-        if t.dtype != torch.int32 or n.dtype != torch.int32 or r.dtype != torch.int32:
+        if t.dtype != _INT or n.dtype != _INT or r.dtype != _INT:
             raise ValueError("page_table, seq_len and row_start must be int32")
         batch, max_pages = t.shape
         if n.shape != (batch,) or r.shape != (batch + 1,) or not (t.is_contiguous() and n.is_contiguous() and r.is_contiguous()):
             raise ValueError("seq_len has an entry per sequence, row_start one more; all are contiguous")
         if not t.get_device() == n.get_device() == r.get_device() == self._device:
             raise ValueError("the sequences' tensors lie on the cache's device")
-        desc = KvCacheDesc(*self._pool, *at[1:], batch, max_pages, s.max_new, s.max_len)
-        object.__setattr__(s, "_checked", (at, desc))
-        return desc
+        return KvCacheDesc.from_buffer_copy(_FIELDS.pack(*self._pool, t.data_ptr(), n.data_ptr(), r.data_ptr(), batch, max_pages, s.max_new, s.max_len))
 
     def _pitch(self, name: str, t: torch.Tensor, rows: int | None, cols: int) -> int:
         shape, stride = t.shape, t.stride()
@@ -106,6 +104,8 @@ class KvCache:
         ld_out = self._pitch("q_out", q_out, rows, heads * HEAD_DIM)
         if rotary is not None and rotary.position is not None and rotary.position.shape != (rows,):
             raise ValueError("position has an entry per row")
+        if rotary is not None and rotary.device not in (None, self._device):
+            raise ValueError("the rotation's tensors lie on the cache's device")
         q = qkv.data_ptr()
         k = q + heads * HEAD_DIM * 2
         with on_device(self._device):

@@ -61,7 +61,7 @@ BAD_CACHES = [dict(head_dim=64), dict(page_size=8), dict(page_size=48), dict(pag
               dict(d_page_table=None), dict(d_seq_len=None), dict(d_row_start=None), dict(d_k=A + 8), dict(d_v=A + 8), dict(kv_heads=40000)]
 
 
-def _append(c, rotary=None, q=A, ld_q=512, q_out=A, ld_q_out=512, heads=4, k=A, v=A, ld_kv=256, rows=3):
+def _append(c, rotary=None, q=A, ld_q=512, q_out=A, ld_q_out=512, heads=4, k=2 * A, v=3 * A, ld_kv=256, rows=3):
     return sfq.lib.sfq_kv_cache_append(C.byref(c) if c is not None else None, C.byref(rotary) if rotary is not None else None, q, ld_q, q_out, ld_q_out,
                                        heads, k, v, ld_kv, rows, None)
 
@@ -96,6 +96,51 @@ def test_append_refuses_rotations(over):
                                   dict(ld_out=516), dict(out=A), dict(q=A + 8), dict(out=2 * A + 2)])
 def test_attention_refuses_operands(over):
     assert _attend(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
+
+
+def test_overlapping_operands_are_refused():
+    # a fused projection: q, k and v in columns of rows of 1024
+    fused = dict(q=A, ld_q=1024, k=A + 512 * 2, v=A + 768 * 2, ld_kv=1024, ld_q_out=1024)
+    for q_out in (A + 16, A - 16, A + 512 * 2 - 16, A + 768 * 2, A + 1024 * 2, A + 1024 * 2 + 512 * 2):
+        assert _append(_cache(), **{**fused, "q_out": q_out}) == sfq.ERR_INVALID_ARGUMENT and b"apart" in sfq.lib.sfq_last_error()
+    assert _append(_cache(), **{**fused, "q_out": A, "ld_q_out": 512}) == sfq.ERR_INVALID_ARGUMENT and b"apart" in sfq.lib.sfq_last_error()
+    # what does not overlap goes on to the next check
+    bad = sfq.RotaryDesc(d_cos=A, d_sin=A, table_rows=5, rotary_dim=24)
+    for q_out, ld in ((A, 1024), (A - 3 * 1024 * 2, 1024), (A + 3 * 1024 * 2, 1024), (2 * A, 512)):
+        assert _append(_cache(), bad, **{**fused, "q_out": q_out, "ld_q_out": ld}) == sfq.ERR_INVALID_ARGUMENT and b"rotary_dim" in sfq.lib.sfq_last_error()
+    for out, ld in ((A + 16, 1024), (A - 16, 1024), (A, 1024), (A, 512), (A + 1024 * 2, 1024)):
+        assert _attend(_cache(), ld_q=1024, out=out, ld_out=ld) == sfq.ERR_INVALID_ARGUMENT and b"overlap" in sfq.lib.sfq_last_error()
+    long = _cache(max_len=100000)
+    assert _attend(long, ld_q=1024, out=A + 512 * 2, ld_out=1024, ws=None) == sfq.ERR_INVALID_ARGUMENT and b"workspace" in sfq.lib.sfq_last_error()
+
+
+def test_scales_that_are_not_finite_are_refused():
+    for scale in (float("nan"), float("inf"), -float("inf")):
+        assert sfq.lib.sfq_kv_cache_attention(C.byref(_cache()), A, 512, 2 * A, 512, 4, 3, scale, A, 1 << 40, None) == sfq.ERR_INVALID_ARGUMENT
+        assert b"scale" in sfq.lib.sfq_last_error()
+
+
+def test_descriptors_follow_their_tensors():
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    cache = KvCache.empty(5, 2, 64, device="cpu")
+    seqs = Sequences(i32(3, 4), i32(3), i32(4), 1, 100)
+    d = cache._desc(seqs)
+    assert C.sizeof(d) == C.sizeof(sfq.KvCacheDesc)
+    want = dict(d_k=cache.k.data_ptr(), d_v=cache.v.data_ptr(), d_k_scale=cache.k_scale.data_ptr(), d_v_scale=cache.v_scale.data_ptr(), num_pages=5, page_size=64,
+                kv_heads=2, head_dim=128, d_page_table=seqs.page_table.data_ptr(), d_seq_len=seqs.seq_len.data_ptr(), d_row_start=seqs.row_start.data_ptr(),
+                batch=3, max_pages=4, max_new=1, max_len=100)
+    assert {k: getattr(d, k) for k in want} == want
+    seqs.page_table.resize_(3, 2)  # the same memory, another shape
+    assert cache._desc(seqs).max_pages == 2
+    seqs.page_table.resize_(2, 2)
+    with pytest.raises(ValueError):
+        cache._desc(seqs)
+    with pytest.raises(AttributeError):  # a rotation's tensors are checked once
+        Rotary(position=i32(3)).position = i32(4)
+    with pytest.raises(ValueError, match="cache's device"):
+        rotary = Rotary(position=i32(3))
+        object.__setattr__(rotary, "device", 0)
+        cache.append(seqs, torch.zeros((3, 8 * 128), dtype=torch.bfloat16), 4, rotary=rotary)
 
 
 def test_attention_refuses_workspaces():

@@ -9,6 +9,9 @@ exp(s - m) is then off by d of itself plus 2^-20, and 2^-11 for its rounding to 
 together twice that, of sum p |v|; sums of T terms in fp32 T 2^-24 at worst; one rounding to bf16, 2^-8."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -610,3 +613,43 @@ def test_decoding_steps(fmt):
         h = check(w1, norm_x(o + x), "swiglu")
         x = check(w2, norm_x(h))
     assert sfq.device_status() == 0
+
+
+FIRST_CALL = """
+import torch
+import slopfab_b200 as sfq
+from slopfab_b200.kv_cache import KvCache, Sequences
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+cache = KvCache.empty(4, 2, 64)
+seqs = Sequences(i32(2, 0).view(1, 2), i32(3), i32(0, 3), 3, 3)
+qkv = torch.randn((3, 8 * 128), device="cuda").to(torch.bfloat16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = cache.attention(seqs, cache.append(seqs, qkv, 4), 4)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, cache.attention(seqs, cache.append(seqs, qkv, 4), 4)) and sfq.device_status() == 0
+print("same")
+"""
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr
+
+
+def test_out_beside_q_in_one_buffer():
+    """q and out are columns of the same rows, q_out is q's place in the projection."""
+    c = Case([2, 1], [40, 33], 2, 2, 16, seed=31).fill([38, 32])
+    wide = torch.randn((3, 4 * D + 2 * D * 2 + 4 * D), device="cuda", generator=c.g).to(torch.bfloat16)
+    n = (4 + 2 * 2) * D
+    fused = wide[:, :n].contiguous()
+    q = c.cache.append(c.seqs, wide[:, :n], 4, q_out=wide[:, : 4 * D])
+    out = c.cache.attention(c.seqs, q, 4, out=wide[:, n:])
+    assert torch.equal(q, fused[:, : 4 * D]) and torch.equal(wide[:, 4 * D: n], fused[:, 4 * D:])
+    assert torch.equal(out, c.cache.attention(c.seqs, fused[:, : 4 * D], 4))
+    with pytest.raises(sfq.SfqError, match="overlap"):
+        c.cache.attention(c.seqs, wide[:, : 4 * D], 4, out=wide[:, D: 5 * D])
+    with pytest.raises(sfq.SfqError, match="apart"):
+        c.cache.append(c.seqs, wide[:, :n], 4, q_out=wide[:, D: 5 * D])
