@@ -33,9 +33,17 @@ int* device_status_word() {
   const int dev = current_device();
   std::lock_guard<std::mutex> lock(g_mutex);
   if (g_status[dev] == nullptr) {
+    // The first use may fall into a capture, of this thread's stream or another's: allocate outside it, and zero on a stream of its own.
     int* p = nullptr;
+    cudaStream_t zeroing = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     cudaError_t e = cudaMalloc(&p, 256);
-    if (e == cudaSuccess) e = cudaMemset(p, 0, 256);
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&zeroing, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, 256, zeroing);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(zeroing);
+    if (zeroing != nullptr) cudaStreamDestroy(zeroing);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) throw std::runtime_error(std::string("sfq: cannot allocate the status word: ") + cudaGetErrorString(e));
     g_status[dev] = p;
   }
