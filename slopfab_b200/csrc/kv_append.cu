@@ -372,6 +372,9 @@ void kv_check(const KvCacheView& c, int head_dim) {
   if (c.kv_heads > 32768) throw std::invalid_argument("kv cache: too many heads");
   if (!c.k || !c.v || !c.k_scale || !c.v_scale || !c.table || !c.seq_len || !c.row_start) throw std::invalid_argument("kv cache: null buffer");
   if (!aligned16(c.k) || !aligned16(c.v)) throw std::invalid_argument("kv cache: the pools must be 16-byte aligned");
+  for (const void* p : {static_cast<const void*>(c.k_scale), static_cast<const void*>(c.v_scale), static_cast<const void*>(c.table), static_cast<const void*>(c.seq_len),
+                        static_cast<const void*>(c.row_start)})
+    if (reinterpret_cast<uintptr_t>(p) % 4 != 0) throw std::invalid_argument("kv cache: scales, page table, lengths and row starts must be 4-byte aligned");
 }
 
 void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendArgs& g, cudaStream_t stream) {
@@ -390,6 +393,7 @@ void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendA
   if (rot.cos != nullptr && (rot.rotary_dim <= 0 || rot.rotary_dim > kKvHeadDim || rot.rotary_dim % 16 != 0 || rot.table_rows <= 0))
     throw std::invalid_argument("kv append: rotary_dim must be a multiple of 16 up to 128, with at least one table row");
   if (!aligned16(rot.cos) || !aligned16(rot.sin) || !aligned16(rot.q_norm) || !aligned16(rot.k_norm)) throw std::invalid_argument("kv append: tables and norm weights must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(rot.position) % 4 != 0) throw std::invalid_argument("kv append: positions must be 4-byte aligned");
   c.status = device_status_word();
   const int page_size = 1 << c.page_shift, pages = (std::min(c.max_new, c.rows) + page_size - 2) / page_size + 1;
   const size_t bytes = size_t(c.rows) * (g.heads * 4 + c.kv_heads * 6) * kKvHeadDim;

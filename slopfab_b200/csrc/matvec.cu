@@ -707,6 +707,7 @@ void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream
   if (!g.x || !g.y || !g.data) throw std::invalid_argument("matvec: null operand");
   if (g.nf4) {
     if (!g.scale || !g.map || !g.nested_map || !g.nested_absmax) throw std::invalid_argument("matvec: nf4 weight without complete double-quant state");
+    if (!aligned(g.map, 4) || !aligned(g.nested_map, 4) || !aligned(g.nested_absmax, 4)) throw std::invalid_argument("matvec: nf4 tables must be 4-byte aligned");
     if (!power_of_two(nf4_block) || nf4_block < 64 || !power_of_two(nf4_nested_block)) throw std::invalid_argument("matvec: nf4 blocks must be powers of two, of 64 elements at least");
     if (g.in % 64 != 0) throw std::invalid_argument("matvec: nf4 needs in_features % 64 == 0");
     if ((size_t(g.out) * g.in) >> 38 != 0) throw std::invalid_argument("matvec: nf4 weight of more than 2^38 elements");
@@ -719,6 +720,7 @@ void linear_matvec(MatvecArgs g, int nf4_block, int nf4_nested_block, cudaStream
   }
   if (g.act == SFQ_ACT_SWIGLU && g.out % 2 != 0) throw std::invalid_argument("matvec: SwiGLU needs an even out_features");
   if (!aligned(g.data, 16) || !aligned(g.x, 16) || !aligned(g.y, 2)) throw std::invalid_argument("matvec: x and the weight must be 16-byte aligned");
+  if (!aligned(g.bias, g.bias_is_bf16 ? 2 : 4)) throw std::invalid_argument("matvec: bias must be aligned to its elements");
   const int cols = g.act == SFQ_ACT_SWIGLU ? g.out / 2 : g.out;
   {
     const auto x0 = reinterpret_cast<uintptr_t>(g.x), x1 = x0 + size_t(g.rows) * g.in * 2, y0 = reinterpret_cast<uintptr_t>(g.y), y1 = y0 + size_t(g.rows) * cols * 2;

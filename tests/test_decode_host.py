@@ -98,6 +98,17 @@ def test_attention_refuses_operands(over):
     assert _attend(_cache(), **over) == sfq.ERR_INVALID_ARGUMENT
 
 
+def test_buffers_off_their_alignment_are_refused():
+    for name in ("d_k_scale", "d_v_scale", "d_page_table", "d_seq_len", "d_row_start"):
+        c = _cache(**{name: A + 2})
+        assert _append(c) == sfq.ERR_INVALID_ARGUMENT and _attend(c) == sfq.ERR_INVALID_ARGUMENT and b"4-byte" in sfq.lib.sfq_last_error()
+    assert _append(_cache(), sfq.RotaryDesc(d_position=A + 2)) == sfq.ERR_INVALID_ARGUMENT and b"4-byte" in sfq.lib.sfq_last_error()
+    for name in ("nf4_quant_map", "nf4_nested_quant_map", "nf4_nested_absmax"):
+        assert _matvec(_nf4(**{name: A + 2})) == sfq.ERR_INVALID_ARGUMENT and b"4-byte" in sfq.lib.sfq_last_error()
+    for at, fmt in ((A + 2, sfq.F32), (A + 1, sfq.BF16)):
+        assert _matvec(_weight(bias=at, bias_format=fmt)) == sfq.ERR_INVALID_ARGUMENT and b"bias" in sfq.lib.sfq_last_error()
+
+
 def test_overlapping_operands_are_refused():
     # a fused projection: q, k and v in columns of rows of 1024
     fused = dict(q=A, ld_q=1024, k=A + 512 * 2, v=A + 768 * 2, ld_kv=1024, ld_q_out=1024)
