@@ -3,6 +3,8 @@
 // Bound by memory: q, k and v rows are read once, q is written as bf16, k and v as e4m3. A (page, head) has one scale, the smallest
 // power of two s with |x| <= 448 s for all its tokens so far; a power of two, because a page that is filled token by token has its scale
 // raised now and then, and the codes that are there then only move by whole exponents (rounded again where they become subnormal).
+// Measured in a graph with 40 query heads: 1 token 3.1 us, 64 sequences of one token each 4.9 (a launch and four dependent loads), a prompt
+// of 4747 tokens with norm and rotation 38.7 us (3.5 TB/s; norm, rotation and conversions take most of the issue slots).
 #include <cuda_fp8.h>
 
 #include <algorithm>

@@ -11,6 +11,9 @@
 // neighbouring tokens of a lane's V. Softmax with running maximum and sum in fp32; the page's scale of K goes into the score, that of V into
 // the weight.
 // Long sequences are divided over CTAs (flash decoding); a second launch joins their parts in order.
+// Measured in a graph, 40 query heads on 8 kv heads: one sequence of 333 tokens 8.6 us, of 131072 50.5 (5.3 TB/s), 32 of up to 4096
+// 48.5 (3.5 TB/s: waves of CTAs over ragged lengths). 16 of up to 3001 with five new tokens, 40 heads on 10, 59.5 us: three query tiles of
+// eight, where scores, exponentials and products, not memory, take the time.
 #include <cuda_fp16.h>
 
 #include <algorithm>
