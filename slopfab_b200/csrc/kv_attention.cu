@@ -11,8 +11,8 @@
 // neighbouring tokens of a lane's V. Softmax with running maximum and sum in fp32; the page's scale of K goes into the score, that of V into
 // the weight.
 // Long sequences are divided over CTAs (flash decoding); a second launch joins their parts in order.
-// Measured in a graph, 40 query heads on 8 kv heads: one sequence of 333 tokens 8.6 us, of 131072 50.5 (5.3 TB/s), 32 of up to 4096
-// 48.5 (3.5 TB/s: waves of CTAs over ragged lengths). 16 of up to 3001 with five new tokens, 40 heads on 10, 59.5 us: three query tiles of
+// Measured in a graph, 40 query heads on 8 kv heads: one sequence of 333 tokens 8.7 us, of 131072 50.9 (5.3 TB/s), 32 of up to 4096
+// 42.0 (4.1 TB/s). 16 of up to 3001 with five new tokens, 40 heads on 10, 51.7 us: three query tiles of
 // eight, where scores, exponentials and products, not memory, take the time.
 #include <cuda_fp16.h>
 
@@ -34,7 +34,7 @@ using namespace ptx;
 
 constexpr int kTile = 64;        // tokens a warp takes at a time
 constexpr int kTileBytes = kTile * kKvHeadDim;  // of K, and of V
-constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen
+constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen, how many parts there are
 constexpr int kMostSplits = 64;
 constexpr int kNarrowSplits = 16;  // parts up to which a warp joins them
 constexpr int kSms = 148;        // the launch is planned for; the workspace can be asked for without a device
@@ -96,8 +96,34 @@ __device__ __noinline__ void note_nan(uint32_t* columns, uint32_t bad, int at, i
   }
 }
 
+// Into how many parts of a sequence's tiles a launch goes. All parts have as many tiles, those of the longest sequence over `even` where the
+// sequences are nearly as long as each other, else over `ragged`; short ones have fewer parts. So all CTAs take about as long, and their
+// number suits the SMs whichever the lengths are.
+struct Splits {
+  int grid, even, ragged;  // grid: the larger one
+};
+__device__ __forceinline__ int length_of(const KvCacheView& c, long long length) {
+  // lengths are 32-bit; the last few thousand of their range are not used, so that sums of places stay in it
+  return int(max(0ll, min(min(length, (long long)c.max_pages << c.page_shift), 0x7FFF0000ll)));
+}
+__device__ __forceinline__ int tiles_of(int length) { return (length + kTile - 1) / kTile; }
+// Tiles of a part. Whole warps.
+__device__ __forceinline__ int tiles_of_part(const KvCacheView& c, const Splits& splits) {
+  int longest = 0;
+  float sum = 0.0f;
+  for (int b = threadIdx.x & 31; b < c.batch; b += 32) {
+    const int tiles = tiles_of(length_of(c, c.seq_len[b]));
+    longest = max(longest, tiles), sum += float(tiles);
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  const int over = sum * 8.0f >= float(longest) * float(c.batch) * 7.0f ? splits.even : splits.ragged;
+  return max(1, (longest + over - 1) / over);
+}
+
 template <int NT, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, int splits) {
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) kv_attention_kernel(KvCacheView c, KvAttentionArgs g, float* parts, Splits splits) {
   constexpr int kCols = NT * 8, kThreads = kWarps * 32;
   // a tile of K [64 tokens][128] and of V [128][64 tokens] for each warp; when they are done, [kWarps][128][kCols + 1] sums
   extern __shared__ __align__(128) uint8_t smem[];
@@ -111,23 +137,26 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
   grid_dependency_release();
   grid_dependency_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, q = lane & 3;
-  const int head = blockIdx.y, split = int(blockIdx.x) % splits;
+  // parts are the slowest of the grid's dimensions, so that those that short sequences lack do not stand in front of any other
+  const int head = int(blockIdx.x) % c.kv_heads, split = blockIdx.z;
   const int page_mask = (1 << c.page_shift) - 1;
 
-  for (int b = blockIdx.z; b < c.batch; b += gridDim.z) {
+  const int each = splits.grid > 1 ? tiles_of_part(c, splits) : INT_MAX;
+  for (int b = int(blockIdx.x) / c.kv_heads; b < c.batch; b += int(gridDim.x) / c.kv_heads) {
     const KvSequence s = kv_sequence(c, b);
-    // Lengths are 32-bit; the last few thousand of their range are not used, so that sums of places stay in it.
-    const int length = int(max(0ll, min(min(s.length, (long long)c.max_pages << c.page_shift), 0x7FFF0000ll)));
+    const int length = length_of(c, s.length), all_tiles = tiles_of(length);
+    const int used = splits.grid > 1 ? max(1, (all_tiles + each - 1) / each) : 1;  // parts of this sequence
+    if (split >= used) continue;
     const int past = int(max(-0x7FFF0000ll, min(s.length, 0x7FFF0000ll) - s.rows));  // tokens in front of the new ones
     const int all_cols = s.rows * g.group;
-    for (int col0 = int(blockIdx.x) / splits * kCols; col0 < all_cols; col0 += int(gridDim.x) / splits * kCols) {
+    for (int col0 = int(blockIdx.y) * kCols; col0 < all_cols; col0 += int(gridDim.y) * kCols) {
       __syncthreads();  // what the tile in front left in shared memory has been read
       if (threadIdx.x < kKvHeadDim) sh_nan[threadIdx.x] = 0;
       // ---- this warp's tiles, the first on its way under the queries
       const int last = min(length, past + min(col0 + kCols - 1, all_cols - 1) / g.group + 1);  // keys that any column sees
       const int first_hidden = past + col0 / g.group + 1;  // ... that one of them does not
-      const int tiles = (max(last, 0) + kTile - 1) / kTile, per_split = (tiles + splits - 1) / splits;
-      const int tile_end = min(tiles, (split + 1) * per_split);
+      const int tiles = (max(last, 0) + kTile - 1) / kTile;
+      const int tile_end = int(min((long long)tiles, (split + 1ll) * each));
       // A tile's pages: lane c holds that of chunk c % 4 of its four chunks of 16 tokens, -1 where there is none.
       auto page_of = [&](int tile) -> int {
         const int t = tile * kTile + q * 16;
@@ -162,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         }
         cp_commit();
       };
-      int tile = split * per_split + warp;
+      int tile = split * each + warp;
       int pages = page_of(tile), next_pages = page_of(tile + kWarps);
       fetch_k(tile, pages);
       fetch_v(tile, pages);
@@ -459,10 +488,10 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         for (int k = 0; k < 4; ++k)
           if (sh_nan[d4 + k] >> col & 1) sum[k] = NAN;
         const int at = col0 + col, row = s.row0 + at / g.group, qh = head * g.group + at % g.group;
-        if (splits > 1) {
-          float* part = parts + ((size_t(row) * g.heads + qh) * splits + split) * kPartFloats;
+        if (splits.grid > 1) {
+          float* part = parts + ((size_t(row) * g.heads + qh) * splits.grid + split) * kPartFloats;
           *reinterpret_cast<float4*>(part + d4) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-          if (d4 == 0) *reinterpret_cast<float4*>(part + 128) = make_float4(mm, ll, any ? 1.0f : 0.0f, 0.0f);
+          if (d4 == 0) *reinterpret_cast<float4*>(part + 128) = make_float4(mm, ll, any ? 1.0f : 0.0f, float(used));
         } else {
           const float inv = any ? (ll == 0.0f ? NAN : 1.0f / ll) : 0.0f;  // keys but no finite score: NaN; no key: zeros
           uint2 v;
@@ -498,14 +527,20 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvCacheView c, KvAttention
       for (int h = 0; h < kEach; ++h) {
         const int i = lane + 32 * h;
         st[h] = i < splits ? *reinterpret_cast<const float4*>(part + i * kPartFloats + 128) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-        mm = fmaxf(mm, st[h].x), any |= st[h].z != 0.0f;
       }
-      const int each = (splits + kWarps - 1) / kWarps, begin = part0 * each, end = min(splits, begin + each);
+      const int each = (splits + kWarps - 1) / kWarps, begin = part0 * each;
       constexpr int kAhead = 4;
       float4 o[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (begin + k < end) o[k] = *reinterpret_cast<const float4*>(part + (begin + k) * kPartFloats + lane * 4);
+        if (begin + k < min(splits, begin + each)) o[k] = *reinterpret_cast<const float4*>(part + (begin + k) * kPartFloats + lane * 4);
+      // The sequence's parts may be fewer than the launch's; what stands in the others' places has been read along and is not used.
+      const int used = int(__shfl_sync(0xffffffffu, st[0].w, 0)), end = min(used, begin + each);
+#pragma unroll
+      for (int h = 0; h < kEach; ++h) {
+        if (lane + 32 * h >= used) st[h] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        mm = fmaxf(mm, st[h].x), any |= st[h].z != 0.0f;
+      }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
       any = __any_sync(0xffffffffu, any);
@@ -553,7 +588,8 @@ __global__ void __launch_bounds__(128) kv_join_kernel(KvCacheView c, KvAttention
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 struct AttentionPlan {
-  int nt, col_tiles, splits, warps;
+  int nt, col_tiles, warps;
+  Splits splits;
 };
 
 // How a launch is divided, from the host's estimates.
@@ -564,18 +600,28 @@ AttentionPlan plan_for(const KvCacheView& c, int heads, int rows) {
   p.col_tiles = int(std::min<long long>((cols + p.nt * 8 - 1) / (p.nt * 8), 4096));
   const long long ctas = (long long)c.batch * c.kv_heads * p.col_tiles;
   // Waves of CTAs times what a CTA takes: about 4 us around its tiles and, with its SM full, 4.5 us for one of a warp's tiles (one query tile
-  // of eight; 6.5 and 10 with two and three), and 2 us for joining. A CTA of eight warps is alone on its SM. 32 sequences of up to 4096
-  // tokens, 8 kv heads: 57.8 / 50.5 / 48.6 / 49.5 / 53.4 us in 1 / 2 / 3 / 4 / 6 parts; one of 131072: 58.6 / 52.8 / 70.7 in 37 / 55 / 64.
+  // of eight; 6.5 and 10 with two and three), and 2 us for joining. A CTA of eight warps is alone on its SM. Sequences of different lengths
+  // are taken to have three quarters of the parts that as many of the longest would have. 32 sequences, 8 kv heads, in 1 .. 6 parts: all of
+  // 4096 tokens 59.3 / 66.3 / 55.4 / 60.2 / 59.0 / 61.7 us, of up to 4096 58.0 / 40.6 / 48.9 / 43.4 / 47.5 / 47.2; 16 of up to 3001 with five
+  // new tokens, 10 kv heads 77.5 / 49.4 / 61.0 / 54.2 / 54.6 / 56.8; one of 131072: 58.6 / 52.8 / 70.7 in 37 / 55 / 64.
   const int per_tile = p.nt == 1 ? 45 : p.nt == 2 ? 65 : 100, tiles = (c.max_len - 1) / kTile + 1;
-  long long best = LLONG_MAX;
-  for (int warps = 4; warps <= 8; warps += 4) {
-    const long long resident = (warps == 4 ? kResident[p.nt] : 1) * kSms;
-    for (int splits = 1; splits <= std::min(kMostSplits, tiles); ++splits) {
-      const long long waves = (ctas * splits + resident - 1) / resident, each = ((tiles + splits - 1) / splits + warps - 1) / warps;
-      const long long cost = waves * (40 + each * per_tile) + (splits > 1 ? 20 : 0);
-      if (cost < best) best = cost, p.splits = splits, p.warps = warps;
+  // The number of parts that takes least, with all of `live` quarters of the longest sequence's parts there.
+  auto best = [&](int live, int most_warps, int& parts, int& warps) {
+    long long least = LLONG_MAX;
+    for (int w = warps; w <= most_warps; w += 4) {
+      const long long resident = (w == 4 ? kResident[p.nt] : 1) * kSms;
+      for (int n = 1; n <= std::min(kMostSplits, tiles); ++n) {
+        const long long waves = (ctas * n * live + 4 * resident - 1) / (4 * resident), each = ((tiles + n - 1) / n + w - 1) / w;
+        const long long cost = waves * (40 + each * per_tile) + (n > 1 ? 20 : 0);
+        if (cost < least) least = cost, parts = n, warps = w;
+      }
     }
-  }
+  };
+  p.warps = 4;
+  best(4, 8, p.splits.even, p.warps);
+  p.splits.ragged = p.splits.even;
+  if (c.batch > 1) best(3, p.warps, p.splits.ragged, p.warps);
+  p.splits.grid = std::max(p.splits.even, p.splits.ragged);
   return p;
 }
 
@@ -585,7 +631,7 @@ static void check_heads(const KvCacheView& c, int heads) {
   if (heads <= 0 || heads > 32768 || heads % c.kv_heads != 0) throw std::invalid_argument("kv attention: heads must be a multiple of kv_heads");
 }
 
-static size_t workspace_of(const AttentionPlan& p, int heads, int rows) { return p.splits > 1 ? size_t(rows) * heads * p.splits * kPartFloats * sizeof(float) : 0; }
+static size_t workspace_of(const AttentionPlan& p, int heads, int rows) { return p.splits.grid > 1 ? size_t(rows) * heads * p.splits.grid * kPartFloats * sizeof(float) : 0; }
 
 size_t kv_attention_workspace_bytes(const KvCacheView& c, int head_dim, int heads, int rows) {
   kv_check(c, head_dim);
@@ -612,17 +658,17 @@ void kv_attention(KvCacheView c, int head_dim, KvAttentionArgs g, float scale, v
   g.scale_log2 = (scale > 0.0f ? scale : 0.08838834764831845f) * 1.4426950408889634f;
   c.status = device_status_word();
   float* parts = static_cast<float*>(workspace);
-  const dim3 grid(p.splits * p.col_tiles, c.kv_heads, std::min(c.batch, 65535));
+  const dim3 grid(c.kv_heads * std::min(c.batch, 65535), p.col_tiles, p.splits.grid);
   const size_t smem = size_t(p.warps) * 2 * kTileBytes;
   const auto kernel = p.warps == 4 ? (p.nt == 1 ? kv_attention_kernel<1, 4> : p.nt == 2 ? kv_attention_kernel<2, 4> : kv_attention_kernel<3, 4>)
                                    : (p.nt == 1 ? kv_attention_kernel<1, 8> : p.nt == 2 ? kv_attention_kernel<2, 8> : kv_attention_kernel<3, 8>);
   reserve_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "kv attention");
   cudaError_t e = launch_overlapped(0, kernel, grid, dim3(p.warps * 32), smem, stream, c, g, parts, p.splits);
-  if (e == cudaSuccess && p.splits > 1) {
-    const bool wide = p.splits > kNarrowSplits;
+  if (e == cudaSuccess && p.splits.grid > 1) {
+    const bool wide = p.splits.grid > kNarrowSplits;
     const long long units = (long long)std::min(c.max_new, c.rows) * g.heads, ctas = wide ? units : (units + 3) / 4;
     e = launch_overlapped(0, wide ? kv_join_kernel<true> : kv_join_kernel<false>, dim3(unsigned(std::min(ctas, 65535ll)), std::min(c.batch, 65535)), dim3(128), 0,
-                          stream, c, g, static_cast<const float*>(parts), p.splits);
+                          stream, c, g, static_cast<const float*>(parts), p.splits.grid);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("kv attention: launch failed: ") + cudaGetErrorString(e));
 }

@@ -653,3 +653,14 @@ def test_out_beside_q_in_one_buffer():
         c.cache.attention(c.seqs, wide[:, : 4 * D], 4, out=wide[:, D: 5 * D])
     with pytest.raises(sfq.SfqError, match="apart"):
         c.cache.append(c.seqs, wide[:, :n], 4, q_out=wide[:, D: 5 * D])
+
+
+@pytest.mark.parametrize("lens", [[2100, 64, 0, 1, 700, 65, 1300], [2000] * 7, [2000, 1990, 1950, 2000, 1900, 1980, 1970], [3000, 0, 0, 0, 0, 0, 5], [1, 0, 1, 1, 0, 1, 1]])
+@pytest.mark.parametrize("max_len", [None, 64, 100000])
+@pytest.mark.parametrize("news", [1, 5])
+def test_sequences_of_all_lengths_in_parts(lens, max_len, news):
+    """Even and ragged batches, divided as the host's and the device's idea of the lengths has it."""
+    counts = [min(news, n) for n in lens]
+    c = Case(counts, lens, 2, 4, 64, seed=41).fill(lens)
+    c.seqs.max_len = max_len or max(lens)
+    c.check_attention(c.q())
