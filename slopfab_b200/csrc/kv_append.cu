@@ -4,7 +4,7 @@
 // power of two s with |x| <= 448 s for all its tokens so far; a power of two, because a page that is filled token by token has its scale
 // raised now and then, and the codes that are there then only move by whole exponents (rounded again where they become subnormal).
 // Measured in a graph with 40 query heads: 1 token 3.1 us, 64 sequences of one token each 4.9 (a launch and four dependent loads), a prompt
-// of 4747 tokens with norm and rotation 38.7 us (3.5 TB/s; norm, rotation and conversions take most of the issue slots).
+// of 4747 tokens with norm and rotation 36.3 us (3.7 TB/s; norm, rotation and conversions take most of the issue slots).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -24,7 +24,7 @@ using namespace ptx;
 constexpr int kThreads = 512;
 constexpr int kLanes = 16;                  // threads of one head's vector, 8 channels each
 constexpr int kAtOnce = kThreads / kLanes;  // vectors a block works on at once
-constexpr int kQueryHeads = 8;              // query heads a block of the page form rotates
+constexpr int kQueryHeads = 4;              // query heads a block of the page form rotates; 4747 tokens of 40 heads 36.3 us, 2 / 6 / 8: 40.8 / 36.9 / 37.9
 constexpr int kFewTokens = 4;               // new tokens of a sequence up to which a warp takes a (page, head)
 constexpr int kHeld = 2;                    // vectors a thread of the page form holds between its two passes
 
@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(128) kv_append_few_kernel(KvCacheView c, Rotar
   }
 }
 
-// Prompts. blockIdx.x: page of the sequence's new tokens; y: sequence; z: a kv head, behind them groups of query heads. A thread takes the
+// Prompts. blockIdx.x: a kv head, behind them groups of query heads; y: sequence; z: page of the sequence's new tokens, so that what runs at
+// a time reads rows of a fused projection whole (with the pages first 38.6 us in place of 36.3). A thread takes the
 // same piece of up to kHeld tokens' vectors, which stay in registers while the block finds the page's scale (pages of more than 64 tokens
 // are computed twice); V goes through shared memory, so that a channel's tokens are stored side by side.
 __global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView
   auto staged = [&](int channel) { return sh_v + channel * (page_size + 4) + (channel >> 5) * 8; };
   const int vector = threadIdx.x / kLanes, l = threadIdx.x & 15;
   const Place at = place_of(rot, l);
-  const bool queries = int(blockIdx.z) >= c.kv_heads;
+  const bool queries = int(blockIdx.x) >= c.kv_heads;
   const __nv_bfloat16* weight = queries ? rot.q_norm : rot.k_norm;
   const bool norm = weight != nullptr;
   float w[8] = {1, 1, 1, 1, 1, 1, 1, 1};
@@ -242,10 +243,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView
     const KvSequence s = kv_sequence(c, b);
     if (s.rows <= 0) continue;
     const long long first_page = max(s.length - s.rows, 0ll) >> c.page_shift, last_page = (s.length - 1) >> c.page_shift;
-    for (long long p = first_page + blockIdx.x; p <= last_page; p += gridDim.x) {
+    for (long long p = first_page + blockIdx.z; p <= last_page; p += gridDim.z) {
       const Run run = run_of(c, s, p);
       if (queries) {
-        const int head0 = (blockIdx.z - c.kv_heads) * kQueryHeads, heads = min(kQueryHeads, g.heads - head0);
+        const int head0 = (blockIdx.x - c.kv_heads) * kQueryHeads, heads = min(kQueryHeads, g.heads - head0);
         for (int j = vector; j - vector < run.tokens; j += kAtOnce) {  // whole warps
           const bool live = j < run.tokens;
           const int i = min(j, run.tokens - 1);
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView
         continue;
       }
       if (run.tokens <= 0) continue;
-      const int head = blockIdx.z, page = kv_page(c, b, p);
+      const int head = blockIdx.x, page = kv_page(c, b, p);
       if (page < 0) continue;
       const size_t block = size_t(page) * c.kv_heads + head;
       uint8_t* const kc = c.k + ((block * kKvHeadDim) << c.page_shift);
@@ -406,7 +407,7 @@ void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendA
   } else {
     const size_t smem = size_t(kKvHeadDim) * (page_size + 4) + 32;
     const int groups = (g.heads + kQueryHeads - 1) / kQueryHeads;
-    e = launch_overlapped(bytes, kv_append_page_kernel, dim3(pages, std::min(c.batch, 65535), c.kv_heads + groups), dim3(kThreads), smem, stream, c, rot, g);
+    e = launch_overlapped(bytes, kv_append_page_kernel, dim3(c.kv_heads + groups, std::min(c.batch, 65535), std::min(pages, 65535)), dim3(kThreads), smem, stream, c, rot, g);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("kv append: launch failed: ") + cudaGetErrorString(e));
 }
