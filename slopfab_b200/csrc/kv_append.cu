@@ -21,11 +21,12 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kThreads = 512;
 constexpr int kLanes = 16;                  // threads of one head's vector, 8 channels each
-constexpr int kAtOnce = kThreads / kLanes;  // vectors a block works on at once
 constexpr int kQueryHeads = 4;              // query heads a block of the page form rotates; 4747 tokens of 40 heads 36.3 us, 2 / 6 / 8: 40.8 / 36.9 / 37.9
-constexpr int kFewTokens = 4;               // new tokens of a sequence up to which a warp takes a (page, head)
+// New tokens of a sequence up to which a warp takes a (page, head), and up to which a block of 128 threads does; for more, one of 512. 64
+// sequences, 40 + 2 x 8 heads: 2 tokens 7.7 us by warps, 6.7 by small blocks; 5 tokens 15.1, 8.0 and 20.3 by large blocks; 16 tokens 43.7, 13.3
+// and 26.5. More than 16 tokens a page would be computed twice in a small block.
+constexpr int kFewTokens = 1, kSomeTokens = 16;
 constexpr int kHeld = 2;                    // vectors a thread of the page form holds between its two passes
 
 // A thread's eight channels of a head lie in two pieces of four: with rotation over 2 h channels, 4 l .. and h + 4 l .. for the first
@@ -139,7 +140,7 @@ __device__ __forceinline__ Run run_of(const KvCacheView& c, const KvSequence& s,
   return {s.row0 + int(begin - past), int(max(0ll, end - begin)), int(begin & ((1 << c.page_shift) - 1)), begin};
 }
 
-// One or a few tokens a sequence: a warp for each (page of the new tokens, sequence, kv head), k in its lower half and v in its upper, and
+// One token a sequence: a warp for each (page of the new tokens, sequence, kv head), k in its lower half and v in its upper, and
 // for each pair of query heads. What takes the time is the chain of dependent loads (sequence, page, scale), so nothing waits for
 // anything else: no block-wide step, one piece of work a warp.
 __global__ void __launch_bounds__(128) kv_append_few_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
@@ -219,11 +220,13 @@ __global__ void __launch_bounds__(128) kv_append_few_kernel(KvCacheView c, Rotar
   }
 }
 
-// Prompts. blockIdx.x: a kv head, behind them groups of query heads; y: sequence; z: page of the sequence's new tokens, so that what runs at
+// Several tokens, prompts. blockIdx.x: a kv head, behind them groups of query heads; y: sequence; z: page of the sequence's new tokens, so that what runs at
 // a time reads rows of a fused projection whole (with the pages first 38.6 us in place of 36.3). A thread takes the
 // same piece of up to kHeld tokens' vectors, which stay in registers while the block finds the page's scale (pages of more than 64 tokens
 // are computed twice); V goes through shared memory, so that a channel's tokens are stored side by side.
-__global__ void __launch_bounds__(kThreads, 2) kv_append_page_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) kv_append_page_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
+  constexpr int kAtOnce = kThreads / kLanes;  // vectors a block works on at once
   grid_dependency_release();
   grid_dependency_wait();
   __shared__ float peaks[2][kThreads / 32];
@@ -407,7 +410,9 @@ void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendA
   } else {
     const size_t smem = size_t(kKvHeadDim) * (page_size + 4) + 32;
     const int groups = (g.heads + kQueryHeads - 1) / kQueryHeads;
-    e = launch_overlapped(bytes, kv_append_page_kernel, dim3(c.kv_heads + groups, std::min(c.batch, 65535), std::min(pages, 65535)), dim3(kThreads), smem, stream, c, rot, g);
+    const int threads = c.max_new <= kSomeTokens ? 128 : 512;
+    e = launch_overlapped(bytes, threads == 128 ? kv_append_page_kernel<128> : kv_append_page_kernel<512>,
+                          dim3(c.kv_heads + groups, std::min(c.batch, 65535), std::min(pages, 65535)), dim3(threads), smem, stream, c, rot, g);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("kv append: launch failed: ") + cudaGetErrorString(e));
 }

@@ -664,3 +664,14 @@ def test_sequences_of_all_lengths_in_parts(lens, max_len, news):
     c = Case(counts, lens, 2, 4, 64, seed=41).fill(lens)
     c.seqs.max_len = max_len or max(lens)
     c.check_attention(c.q())
+
+
+@pytest.mark.parametrize("most", [1, 2, 5, 16, 17, 40])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_some_tokens(most, page, norm):
+    """Each form of the launch, with sequences of fewer tokens and of none, over page borders."""
+    counts = [most, 1, 0, max(most - 1, 1), most, (most + 1) // 2]
+    past = [0, page - 1, 7, page - 2, 3 * page - most // 2, page]
+    c = Case(counts, [a + b for a, b in zip(counts, past)], 2, 3, page, seed=51).fill(past)
+    check_append(c, new_qkv(c), 96, norm)
