@@ -99,9 +99,11 @@ class KvCache:
         """Stores k and v of the fused projection qkv [rows, (heads + 2 kv_heads) * 128] and returns q, normed and rotated
         (q_out [rows, heads * 128]; pass a view of qkv's first columns to have it in place)."""
         ld, rows = self._pitch("qkv", qkv, None, (heads + 2 * self.kv_heads) * HEAD_DIM), qkv.shape[0]
+        ld_out = heads * HEAD_DIM
         if q_out is None:
-            q_out = torch.empty((rows, heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
-        ld_out = self._pitch("q_out", q_out, rows, heads * HEAD_DIM)
+            q_out = qkv.new_empty((rows, ld_out))
+        else:
+            ld_out = self._pitch("q_out", q_out, rows, ld_out)
         if rotary is not None and rotary.position is not None and rotary.position.shape != (rows,):
             raise ValueError("position has an entry per row")
         if rotary is not None and rotary.device not in (None, self._device):
@@ -119,9 +121,11 @@ class KvCache:
         """softmax(q K^T scale) V of the new tokens' q [rows, heads * 128] over the cache, causal among them; scale 0 means 1 / sqrt(128).
         The workspace is the call's own, so that calls on several streams and captured graphs share none."""
         ld, rows = self._pitch("q", q, None, heads * HEAD_DIM), q.shape[0]
+        ld_out = heads * HEAD_DIM
         if out is None:
-            out = torch.empty((rows, heads * HEAD_DIM), dtype=torch.bfloat16, device=self.device)
-        ld_out = self._pitch("out", out, rows, heads * HEAD_DIM)
+            out = q.new_empty((rows, ld_out))
+        else:
+            ld_out = self._pitch("out", out, rows, ld_out)
         with on_device(self._device):
             desc, n = self._desc(s), C.c_size_t()
             check(lib.sfq_kv_cache_attention_workspace_bytes(C.byref(desc), heads, rows, C.byref(n)))
