@@ -675,3 +675,10 @@ def test_append_some_tokens(most, page, norm):
     past = [0, page - 1, 7, page - 2, 3 * page - most // 2, page]
     c = Case(counts, [a + b for a, b in zip(counts, past)], 2, 3, page, seed=51).fill(past)
     check_append(c, new_qkv(c), 96, norm)
+
+
+@pytest.mark.parametrize("even", [False, True])
+def test_more_sequences_than_lanes(even):
+    lens = [700 if even else (37 * i * i) % 900 for i in range(70)]
+    c = Case([min(1, n) for n in lens], lens, 1, 4, 64, seed=61).fill(lens)
+    c.check_attention(c.q())
