@@ -202,3 +202,23 @@ def test_python_faces_refuse_what_does_not_fit():
         Rotary(q_norm=torch.ones(64, dtype=torch.bfloat16))
     with pytest.raises(ValueError):
         Rotary(torch.zeros((4, 48)), torch.zeros((4, 48)), position=torch.zeros(3))
+
+
+def _host_cache():
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    return KvCache.empty(5, 2, 64, device="cpu"), Sequences(i32(3, 4), i32(3), i32(4), 1, 100)
+
+
+def test_rows_that_overlap_are_refused():
+    """A row that is repeated by a stride of 0, and windows that slide over a buffer: their pitch is less than a row."""
+    cache, seqs = _host_cache()
+    wide = torch.zeros(3 * 8 * 128, dtype=torch.bfloat16)
+    qkv, q, out = wide.view(3, -1), wide.view(3, -1)[:, :512], torch.zeros((3, 512), dtype=torch.bfloat16)
+    for n, call in ((8 * 128, lambda t: cache.append(seqs, t, 4)), (512, lambda t: cache.append(seqs, qkv, 4, q_out=t)),
+                    (512, lambda t: cache.attention(seqs, t, 4)), (512, lambda t: cache.attention(seqs, q, 4, out=t))):
+        for bad in (wide[:n].expand(3, n), wide.as_strided((3, n), (n // 2, 1)), wide.as_strided((3, n), (n - 8, 1))):
+            with pytest.raises(ValueError, match="overlap"):
+                call(bad)
+    for good in (q, out):  # these go on to the next check
+        with pytest.raises(ValueError, match="CUDA device"):
+            cache.attention(seqs, good, 4)
