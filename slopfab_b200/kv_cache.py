@@ -93,9 +93,11 @@ class KvCache:
         shape, stride = t.shape, t.stride()
         if t.dtype != torch.bfloat16 or len(shape) != 2 or shape[1] != cols or stride[1] != 1 or t.get_device() != self._device or rows not in (None, shape[0]):
             raise ValueError(f"{name} must be bf16 [{'rows' if rows is None else rows}, {cols}] with contiguous rows, on the cache's device")
-        if shape[0] > 1 and stride[0] < cols:
+        if shape[0] <= 1:
+            return cols  # a single row may have any stride
+        if stride[0] < cols:
             raise ValueError(f"{name}'s rows overlap: they lie {stride[0]} elements apart and have {cols}")
-        return max(stride[0], cols)  # a single row may have any stride
+        return stride[0]
 
     def append(self, s: Sequences, qkv: torch.Tensor, heads: int, q_out: torch.Tensor | None = None, rotary: Rotary | None = None) -> torch.Tensor:
         """Stores k and v of the fused projection qkv [rows, (heads + 2 kv_heads) * 128] and returns q, normed and rotated

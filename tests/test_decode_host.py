@@ -222,3 +222,12 @@ def test_rows_that_overlap_are_refused():
     for good in (q, out):  # these go on to the next check
         with pytest.raises(ValueError, match="CUDA device"):
             cache.attention(seqs, good, 4)
+
+
+def test_a_single_row_has_no_pitch():
+    """The stride of one row says nothing: it may be odd, less than the row, or more than 32 bits hold."""
+    cache, _ = _host_cache()
+    wide = torch.zeros(2 * 2058, dtype=torch.bfloat16).view(2, 2058)
+    for row in (wide[:1, :512], wide[0, :512].expand(1, 512), wide[0].as_strided((1, 512), (1, 1)), wide[0].as_strided((1, 512), (1 << 40, 1))):
+        assert cache._pitch("q", row, 1, 512) == 512, row.stride()
+    assert cache._pitch("q", wide[:, :512], 2, 512) == 2058

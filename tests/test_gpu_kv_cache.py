@@ -682,3 +682,19 @@ def test_more_sequences_than_lanes(even):
     lens = [700 if even else (37 * i * i) % 900 for i in range(70)]
     c = Case([min(1, n) for n in lens], lens, 1, 4, 64, seed=61).fill(lens)
     c.check_attention(c.q())
+
+
+def test_a_row_of_a_buffer_of_odd_width():
+    """One token whose q, k, v, q_out and out are rows of buffers with pitches that several rows could not have."""
+    c = Case([1], [90], 2, 2, 64, seed=71).fill([89])
+    d = Case([1], [90], 2, 2, 64, seed=71).fill([89])
+    qkv = new_qkv(c)
+    rows = [torch.full((2, n * D + 10), 3.0, dtype=torch.bfloat16, device="cuda") for n in (8, 4, 4)]
+    rows[0][0, : 8 * D] = qkv[0]
+    q = c.cache.append(c.seqs, rows[0][:1, : 8 * D], 4, q_out=rows[1][:1, : 4 * D])
+    out = c.cache.attention(c.seqs, q, 4, out=rows[2][:1, : 4 * D])
+    want = d.cache.append(d.seqs, qkv, 4)
+    assert torch.equal(q, want) and torch.equal(out, d.cache.attention(d.seqs, want, 4))
+    for r in rows[1:]:
+        assert bool((r[0, 4 * D:] == 3).all()) and bool((r[1] == 3).all())
+    assert sfq.device_status() == 0
