@@ -97,6 +97,8 @@ class KvCache:
             return cols  # a single row may have any stride
         if stride[0] < cols:
             raise ValueError(f"{name}'s rows overlap: they lie {stride[0]} elements apart and have {cols}")
+        if stride[0] >= 1 << 31:
+            raise ValueError(f"{name}'s rows lie {stride[0]} elements apart; the library takes a pitch of 32 bits")
         return stride[0]
 
     def append(self, s: Sequences, qkv: torch.Tensor, heads: int, q_out: torch.Tensor | None = None, rotary: Rotary | None = None) -> torch.Tensor:

@@ -231,3 +231,11 @@ def test_a_single_row_has_no_pitch():
     for row in (wide[:1, :512], wide[0, :512].expand(1, 512), wide[0].as_strided((1, 512), (1, 1)), wide[0].as_strided((1, 512), (1 << 40, 1))):
         assert cache._pitch("q", row, 1, 512) == 512, row.stride()
     assert cache._pitch("q", wide[:, :512], 2, 512) == 2058
+
+
+def test_pitches_of_more_than_32_bits_are_refused():
+    """ctypes would pass on their low 32 bits, 512 here."""
+    cache, _ = _host_cache()
+    for stride in ((1 << 32) + 512, 1 << 31):
+        with pytest.raises(ValueError, match="32 bits"):
+            cache._pitch("q", torch.empty((2, stride), dtype=torch.bfloat16, device="meta")[:, :512], 2, 512)
