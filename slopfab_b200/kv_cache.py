@@ -12,6 +12,7 @@ from .linear import on_device, raw_stream
 
 HEAD_DIM = 128
 _INT = torch.int32
+_POOL = ("k", "v", "k_scale", "v_scale")
 _FIELDS = struct.Struct("4P4i3P4i")  # sfq_kv_cache; packed at once, which takes a quarter of the time of ctypes' constructor
 
 
@@ -57,9 +58,20 @@ class Rotary:
 
 class KvCache:
     """Pages of keys and values in e4m3 with one scale per (page, head): k uint8 [pages, kv_heads, page_size, 128], v uint8 [pages,
-    kv_heads, 128, page_size], scales fp32 [pages, kv_heads]. The tensors are the caller's; `KvCache.empty` makes them."""
+    kv_heads, 128, page_size], scales fp32 [pages, kv_heads]. The tensors are the caller's; `KvCache.empty` makes them. They may be
+    replaced, all four for a pool of another size: a call takes them as they then are."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._check_pool()
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if name in _POOL:
+            object.__setattr__(self, "_pool", None)
+
+    def _check_pool(self) -> None:
+        k, v, k_scale, v_scale = self.k, self.v, self.k_scale, self.v_scale
         pages, kv_heads, page_size, dim = k.shape
         if k.dtype != torch.uint8 or v.dtype != torch.uint8 or v.shape != (pages, kv_heads, dim, page_size):
             raise ValueError("k must be uint8 [pages, kv_heads, page_size, 128] and v [pages, kv_heads, 128, page_size]")
@@ -68,9 +80,8 @@ class KvCache:
                 raise ValueError("scales must be fp32 [pages, kv_heads]")
         if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
             raise ValueError("the pools and their scales lie on one device")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.kv_heads, self.device, self._device = kv_heads, k.device, k.get_device()
-        self._pool = (ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, page_size, kv_heads, dim)
+        self._pool, self._shape = (ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, page_size, kv_heads, dim), k.shape
 
     @staticmethod
     def empty(pages: int, kv_heads: int, page_size: int = 64, device="cuda") -> "KvCache":
@@ -78,7 +89,16 @@ class KvCache:
         v = torch.zeros((pages, kv_heads, HEAD_DIM, page_size), dtype=torch.uint8, device=device)
         return KvCache(k, v, *(torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)))
 
-    def _desc(self, s: Sequences) -> KvCacheDesc:
+    def _pool_now(self) -> tuple:
+        pool, k = self._pool, self.k
+        if pool is None or k.data_ptr() != pool[0] or self.v.data_ptr() != pool[1] or self.k_scale.data_ptr() != pool[2] or self.v_scale.data_ptr() != pool[3] or k.shape != self._shape:
+            self._check_pool()  # a tensor was replaced, or has got other memory
+            pool = self._pool
+        return pool
+
+    def _desc(self, s: Sequences, pool: tuple | None = None) -> KvCacheDesc:
+        if pool is None:
+            pool = self._pool_now()
         t, n, r = s.page_table, s.seq_len, s.row_start
         if t.dtype != _INT or n.dtype != _INT or r.dtype != _INT:
             raise ValueError("page_table, seq_len and row_start must be int32")
@@ -87,7 +107,7 @@ class KvCache:
             raise ValueError("seq_len has an entry per sequence, row_start one more; all are contiguous")
         if not t.get_device() == n.get_device() == r.get_device() == self._device:
             raise ValueError("the sequences' tensors lie on the cache's device")
-        return KvCacheDesc.from_buffer_copy(_FIELDS.pack(*self._pool, t.data_ptr(), n.data_ptr(), r.data_ptr(), batch, max_pages, s.max_new, s.max_len))
+        return KvCacheDesc.from_buffer_copy(_FIELDS.pack(*pool, t.data_ptr(), n.data_ptr(), r.data_ptr(), batch, max_pages, s.max_new, s.max_len))
 
     def _pitch(self, name: str, t: torch.Tensor, rows: int | None, cols: int) -> int:
         shape, stride = t.shape, t.stride()
@@ -104,6 +124,7 @@ class KvCache:
     def append(self, s: Sequences, qkv: torch.Tensor, heads: int, q_out: torch.Tensor | None = None, rotary: Rotary | None = None) -> torch.Tensor:
         """Stores k and v of the fused projection qkv [rows, (heads + 2 kv_heads) * 128] and returns q, normed and rotated
         (q_out [rows, heads * 128]; pass a view of qkv's first columns to have it in place)."""
+        pool = self._pool_now()
         ld, rows = self._pitch("qkv", qkv, None, (heads + 2 * self.kv_heads) * HEAD_DIM), qkv.shape[0]
         ld_out = heads * HEAD_DIM
         if q_out is None:
@@ -117,7 +138,7 @@ class KvCache:
         q = qkv.data_ptr()
         k = q + heads * HEAD_DIM * 2
         with on_device(self._device):
-            status = lib.sfq_kv_cache_append(C.byref(self._desc(s)), C.byref(rotary.desc) if rotary is not None else None, q, ld, q_out.data_ptr(), ld_out,
+            status = lib.sfq_kv_cache_append(C.byref(self._desc(s, pool)), C.byref(rotary.desc) if rotary is not None else None, q, ld, q_out.data_ptr(), ld_out,
                                              heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, raw_stream(self._device))
         if status:
             check(status)
@@ -126,6 +147,7 @@ class KvCache:
     def attention(self, s: Sequences, q: torch.Tensor, heads: int, out: torch.Tensor | None = None, scale: float = 0.0) -> torch.Tensor:
         """softmax(q K^T scale) V of the new tokens' q [rows, heads * 128] over the cache, causal among them; scale 0 means 1 / sqrt(128).
         The workspace is the call's own, so that calls on several streams and captured graphs share none."""
+        pool = self._pool_now()
         ld, rows = self._pitch("q", q, None, heads * HEAD_DIM), q.shape[0]
         ld_out = heads * HEAD_DIM
         if out is None:
@@ -133,7 +155,7 @@ class KvCache:
         else:
             ld_out = self._pitch("out", out, rows, ld_out)
         with on_device(self._device):
-            desc, n = self._desc(s), C.c_size_t()
+            desc, n = self._desc(s, pool), C.c_size_t()
             check(lib.sfq_kv_cache_attention_workspace_bytes(C.byref(desc), heads, rows, C.byref(n)))
             ws = torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
             status = lib.sfq_kv_cache_attention(C.byref(desc), q.data_ptr(), ld, out.data_ptr(), ld_out, heads, rows, scale, ws.data_ptr() if n.value else None,

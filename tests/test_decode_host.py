@@ -239,3 +239,40 @@ def test_pitches_of_more_than_32_bits_are_refused():
     for stride in ((1 << 32) + 512, 1 << 31):
         with pytest.raises(ValueError, match="32 bits"):
             cache._pitch("q", torch.empty((2, stride), dtype=torch.bfloat16, device="meta")[:, :512], 2, 512)
+
+
+def test_the_pool_follows_its_tensors():
+    """A pool whose tensors are replaced, grown or given other memory: a call never goes to the memory of before, and what no longer
+    fits together is refused."""
+    cache, seqs = _host_cache()
+    larger = KvCache.empty(9, 2, 64, device="cpu")
+    tensors = lambda c: (c.k, c.v, c.k_scale, c.v_scale)  # noqa: E731
+    addresses = lambda d: (d.d_k, d.d_v, d.d_k_scale, d.d_v_scale)  # noqa: E731
+    cache.k = larger.k
+    with pytest.raises(ValueError):  # the other three have five pages
+        cache._desc(seqs)
+    with pytest.raises(ValueError):
+        cache.append(seqs, torch.zeros((3, 8 * 128), dtype=torch.bfloat16), 4)
+    cache.v, cache.k_scale, cache.v_scale = larger.v, larger.k_scale, larger.v_scale
+    d = cache._desc(seqs)
+    assert addresses(d) == tuple(t.data_ptr() for t in tensors(larger)) and d.num_pages == 9
+    cache.k_scale = torch.zeros((9, 2), dtype=torch.float64)
+    with pytest.raises(ValueError):
+        cache._desc(seqs)
+    cache.k_scale = larger.k_scale
+    cache.k_scale *= 2  # the same tensor
+    for t in tensors(cache):  # the same tensors, other memory
+        t.set_(t.clone())
+        d = cache._desc(seqs)
+        assert addresses(d) == tuple(u.data_ptr() for u in tensors(cache)) and d.num_pages == 9
+    cache.k.resize_(11, 2, 64, 128)
+    with pytest.raises(ValueError):
+        cache._desc(seqs)
+    cache.k.resize_(3, 2, 64, 128)  # the same memory, fewer pages than the others
+    with pytest.raises(ValueError):
+        cache._desc(seqs)
+    few = KvCache.empty(4, 3, 16, device="cpu")
+    cache.k, cache.v, cache.k_scale, cache.v_scale = tensors(few)
+    assert (cache._desc(seqs).kv_heads, cache._desc(seqs).page_size) == (3, 16) and cache.kv_heads == 3
+    with pytest.raises(ValueError, match="CUDA device"):  # rows of the heads that there are now
+        cache.append(seqs, torch.zeros((3, 9 * 128), dtype=torch.bfloat16), 3)
