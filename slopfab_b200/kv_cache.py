@@ -51,9 +51,22 @@ class Rotary:
         devices = {t.get_device() for t in (self.cos, self.sin, self.position, self.q_norm, self.k_norm) if t is not None}
         if len(devices) > 1:
             raise ValueError("the tables, positions and norm weights lie on one device")
-        rows, half = self.cos.shape if self.cos is not None else (0, 0)
+        shape = self.cos.shape if self.cos is not None else (0, 0)
+        rows, half = shape
         object.__setattr__(self, "device", devices.pop() if devices else None)
         object.__setattr__(self, "desc", RotaryDesc(ptr(self.cos), ptr(self.sin), ptr(self.position), rows, 2 * half, ptr(self.q_norm), ptr(self.k_norm), self.eps))
+        object.__setattr__(self, "_shape", shape)
+        object.__setattr__(self, "_held", [(t, t.data_ptr()) for t in (self.cos, self.sin, self.position, self.q_norm, self.k_norm) if t is not None])
+
+    def _desc_now(self) -> RotaryDesc:
+        for t, at in self._held:
+            if t.data_ptr() != at:  # the tensor has got other memory
+                self.__post_init__()
+                break
+        else:
+            if self.cos is not None and self.cos.shape != self._shape:
+                self.__post_init__()
+        return self.desc
 
 
 class KvCache:
@@ -131,14 +144,17 @@ class KvCache:
             q_out = qkv.new_empty((rows, ld_out))
         else:
             ld_out = self._pitch("q_out", q_out, rows, ld_out)
-        if rotary is not None and rotary.position is not None and rotary.position.shape != (rows,):
-            raise ValueError("position has an entry per row")
-        if rotary is not None and rotary.device not in (None, self._device):
-            raise ValueError("the rotation's tensors lie on the cache's device")
+        rotation = None
+        if rotary is not None:
+            rotation = rotary._desc_now()
+            if rotary.position is not None and rotary.position.shape != (rows,):
+                raise ValueError("position has an entry per row")
+            if rotary.device not in (None, self._device):
+                raise ValueError("the rotation's tensors lie on the cache's device")
         q = qkv.data_ptr()
         k = q + heads * HEAD_DIM * 2
         with on_device(self._device):
-            status = lib.sfq_kv_cache_append(C.byref(self._desc(s, pool)), C.byref(rotary.desc) if rotary is not None else None, q, ld, q_out.data_ptr(), ld_out,
+            status = lib.sfq_kv_cache_append(C.byref(self._desc(s, pool)), C.byref(rotation) if rotation is not None else None, q, ld, q_out.data_ptr(), ld_out,
                                              heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, raw_stream(self._device))
         if status:
             check(status)

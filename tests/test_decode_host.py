@@ -276,3 +276,23 @@ def test_the_pool_follows_its_tensors():
     assert (cache._desc(seqs).kv_heads, cache._desc(seqs).page_size) == (3, 16) and cache.kv_heads == 3
     with pytest.raises(ValueError, match="CUDA device"):  # rows of the heads that there are now
         cache.append(seqs, torch.zeros((3, 9 * 128), dtype=torch.bfloat16), 3)
+
+
+def test_a_rotation_follows_its_tensors():
+    """Tables, positions and norm weights that are given other memory, as a module's are when its data is replaced."""
+    bf16 = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    r = Rotary(torch.zeros((40, 48)), torch.zeros((40, 48)), torch.zeros(3, dtype=torch.int32), bf16(128), bf16(128))
+    names = ("cos", "sin", "position", "q_norm", "k_norm")
+    assert r._desc_now() is r.desc
+    for name in names:
+        t = getattr(r, name)
+        t.data = t.clone()
+        d = r._desc_now()
+        assert [getattr(d, "d_" + n) for n in names] == [getattr(r, n).data_ptr() for n in names]
+    r.sin.resize_(20, 48)
+    r.cos.resize_(20, 48)  # the same memory, fewer rows
+    assert r._desc_now().table_rows == 20
+    r.cos.resize_(60, 48)
+    cache, seqs = _host_cache()
+    with pytest.raises(ValueError, match="cos and sin"):
+        cache.append(seqs, bf16(3, 8 * 128), 4, rotary=r)
