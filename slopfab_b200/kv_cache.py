@@ -93,6 +93,9 @@ class KvCache:
                 raise ValueError("scales must be fp32 [pages, kv_heads]")
         if len({t.device for t in (k, v, k_scale, v_scale)}) != 1:
             raise ValueError("the pools and their scales lie on one device")
+        places = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (k, v, k_scale, v_scale))
+        if any(end > start for (_, end), (start, _) in zip(places, places[1:])):
+            raise ValueError("k, v and their scales lie apart")
         self.kv_heads, self.device, self._device = kv_heads, k.device, k.get_device()
         self._pool, self._shape = (ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, page_size, kv_heads, dim), k.shape
 

@@ -296,3 +296,16 @@ def test_a_rotation_follows_its_tensors():
     cache, seqs = _host_cache()
     with pytest.raises(ValueError, match="cos and sin"):
         cache.append(seqs, bf16(3, 8 * 128), 4, rotary=r)
+
+
+def test_pools_that_share_memory_are_refused():
+    """With pages of 128 tokens K and V have the same shape, and one tensor could be given for both; scales always have."""
+    cache = KvCache.empty(5, 2, 128, device="cpu")
+    both = torch.zeros((6, 2, 128, 128), dtype=torch.uint8)
+    scales = torch.zeros(19)
+    for bad in ((cache.k, cache.k, cache.k_scale, cache.v_scale), (cache.k, cache.v, cache.k_scale, cache.k_scale), (both[:5], both[1:], cache.k_scale, cache.v_scale),
+                (cache.k, cache.v, scales[9:].view(5, 2), scales[:10].view(5, 2))):
+        with pytest.raises(ValueError, match="apart"):
+            KvCache(*bad)
+    scales = torch.zeros(20)
+    KvCache(cache.k, cache.v, scales[10:].view(5, 2), scales[:10].view(5, 2))  # side by side
