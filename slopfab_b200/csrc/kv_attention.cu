@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
               for (int e = 0; e < 4; ++e) o[d][n][e] *= keep[n][e & 1];
         }
         // Where the references lie near each other, as they do unless pages' scales differ by a great deal, the second weight is the first
-        // times a factor.
+        // times a factor. Differences of scores come before e: they are exact where they count, while a large score and e is not.
         float factor[NT][2];
         bool near = true;
 #pragma unroll
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             ref[e] = m[n][e] == -INFINITY ? 0.0f : m[n][e];
-            ref_v[e] = e_mine - (mv[n][e] == -INFINITY ? 0.0f : mv[n][e]);
+            ref_v[e] = mv[n][e] == -INFINITY ? 0.0f : mv[n][e];
           }
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
             for (int e = 0; e < 4; ++e) {
               w[e] = exp2_fast(sc[t][n][e] - ref[e & 1]);
               l[n][e & 1] += w[e];
-              w[e] = near ? w[e] * factor[n][e & 1] : exp2_fast(sc[t][n][e] + ref_v[e & 1]) * frac;
+              w[e] = near ? w[e] * factor[n][e & 1] : exp2_fast(sc[t][n][e] - ref_v[e & 1] + e_mine) * frac;
             }
             p[t][n][0] = transpose8x8(half_pair(w[0], w[1]));
             p[t][n][1] = transpose8x8(half_pair(w[2], w[3]));

@@ -698,3 +698,25 @@ def test_a_row_of_a_buffer_of_odd_width():
     for r in rows[1:]:
         assert bool((r[0, 4 * D:] == 3).all()) and bool((r[1] == 3).all())
     assert sfq.device_status() == 0
+
+
+@pytest.mark.parametrize("size", [2.0 ** 15, 2.0 ** 21, 2.0 ** 24, 2.0 ** 25])
+@pytest.mark.parametrize("shift", [-60, 0, 60])
+def test_scores_whose_last_place_is_an_octave_and_more(size, shift):
+    """Scores of up to `size` octaves, in fp32 steps of 2^-24 of that: the key with all the weight is the result, whatever its page's scale."""
+    n = 200
+    c = Case([1], [n], 1, 2, 16, seed=82).fill([n])
+    page = c.table[0, : -(-n // 16)].long()
+    c.cache.v_scale[page] *= 2.0 ** shift
+    c.v *= 2.0 ** shift
+    c.cache.k_scale[page] = 1.0
+    c.cache.k[page] = 0
+    one = torch.tensor([1.0, 0.875]).to(torch.float8_e4m3fn).view(torch.uint8).tolist()
+    for at in range(0, n, 7):  # this key is alone at the top
+        c.cache.k[page[:, None], 0, torch.arange(16, device="cuda"), 0] = one[1]
+        c.cache.k[page[at // 16], 0, at % 16, 0] = one[0]
+        q = torch.zeros_like(c.q())
+        q[0, 0], q[0, D] = 1.0, 1.0
+        got = c.cache.attention(c.seqs, q, 2, scale=size * math.log(2))
+        want = c.v[0, 0, at].to(torch.bfloat16)
+        assert torch.equal(got.view(2, D), want.expand(2, D)), at
