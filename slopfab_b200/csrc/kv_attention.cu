@@ -356,17 +356,18 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         }
         // Where the references lie near each other, as they do unless pages' scales differ by a great deal, the second weight is the first
         // times a factor. Differences of scores come before e: they are exact where they count, while a large score and e is not.
+        // Which way a weight is made depends on nothing but its own query and page, so that no query changes another's bits.
         float factor[NT][2];
-        bool near = true;
+        uint32_t far = 0;  // bit 2 n + e
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float between = m[n][e] == -INFINITY ? 0.0f : m[n][e] - mv[n][e] + e_mine;
-            near &= fabsf(between) < 60.0f;
+            if (!(fabsf(between) < 60.0f)) far |= 1u << (2 * n + e);  // NaN, too
             factor[n][e] = exp2_fast(between) * frac;
           }
-        near = __all_sync(0xffffffffu, near);
+        const bool near = __all_sync(0xffffffffu, far == 0);
         uint32_t p[4][NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
             for (int e = 0; e < 4; ++e) {
               w[e] = exp2_fast(sc[t][n][e] - ref[e & 1]);
               l[n][e & 1] += w[e];
-              w[e] = near ? w[e] * factor[n][e & 1] : exp2_fast(sc[t][n][e] - ref_v[e & 1] + e_mine) * frac;
+              w[e] = near || (far >> (2 * n + (e & 1)) & 1) == 0 ? w[e] * factor[n][e & 1] : exp2_fast(sc[t][n][e] - ref_v[e & 1] + e_mine) * frac;
             }
             p[t][n][0] = transpose8x8(half_pair(w[0], w[1]));
             p[t][n][1] = transpose8x8(half_pair(w[2], w[3]));

@@ -720,3 +720,19 @@ def test_scores_whose_last_place_is_an_octave_and_more(size, shift):
         got = c.cache.attention(c.seqs, q, 2, scale=size * math.log(2))
         want = c.v[0, 0, at].to(torch.bfloat16)
         assert torch.equal(got.view(2, D), want.expand(2, D)), at
+
+
+@pytest.mark.parametrize("news,group", [(1, 5), (3, 4), (40, 5)])
+def test_heads_and_tokens_stand_for_themselves(news, group):
+    """An infinite or NaN query, and one whose scores lie far from the others', changes no bit of the queries beside it, which share
+    its tile."""
+    c = Case([news] * 8, [100 + i for i in range(8)], 8, group, 32, seed=83).fill([100 + i for i in range(8)])
+    for seed in range(8):
+        q = c.q()
+        clean = c.check_attention(q).view(-1, 8, group, D)
+        for bad in (float("inf"), float("nan"), 3e4, -3e4):
+            other = q.clone()
+            other.view(-1, 8, group, D)[:, :, seed % group, 9] = bad
+            got = c.cache.attention(c.seqs, other, c.heads).view(-1, 8, group, D)
+            got[:, :, seed % group] = clean[:, :, seed % group]
+            assert torch.equal(got, clean), (seed, bad, int((got != clean).sum()))
