@@ -517,7 +517,8 @@ SFQ_API int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rot
 
 /* out[rows, heads * 128] = softmax(q K^T scale) V over the cache: the i-th of a sequence's n new tokens sees its first length - n + i + 1
  * keys; query head h reads kv head h / (heads / kv_heads). scale <= 0 selects 1 / sqrt(128). out and q lie apart. A row that sees no key is zero; a NaN or +inf
- * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Slots behind a sequence's length may hold
+ * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Scores, weights and sums are fp32; in front
+ * of V a weight is rounded to fp16, relative to the largest weight near it: to eleven bits down to 2^-29 of that one, to zero below 2^-40. Slots behind a sequence's length may hold
  * anything. The workspace is scratch of one call and needs no initialisation; it may be null where
  * sfq_kv_cache_attention_workspace_bytes gives 0. */
 SFQ_API int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, int rows, size_t* out);

@@ -34,6 +34,7 @@ using namespace ptx;
 
 constexpr int kTile = 64;        // tokens a warp takes at a time
 constexpr int kTileBytes = kTile * kKvHeadDim;  // of K, and of V
+constexpr float kLift = 15.0f, kLower = 0x1p-15f;  // the largest weight of the second product is below 2^kLift, see there
 constexpr int kPartFloats = 132; // of a divided row and head: O [128], maximum, sum, whether any key was seen, how many parts there are
 constexpr int kMostSplits = 64;
 constexpr int kNarrowSplits = 16;  // parts up to which a warp joins them
@@ -299,8 +300,10 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         const bool whole = __all_sync(0xffffffffu, page >= 0) && t0 + kTile <= min(first_hidden, length);
         const int mine = t0 + (gq >> 1) * 16 + (gq & 1);  // token of row gq of MMA 0; row gq + 8 is two behind, MMA t four t
         // The weights of the second product are p vs = exp2(score + e) (vs / 2^e) with vs / 2^e in [0.5, 1), over their own running
-        // reference mv, the largest score + e: a page of small values that has all the weight keeps its bits beside one of large values
-        // that has none.
+        // reference mv, the largest score + e less kLift: a page of small values that has all the weight keeps its bits beside one of
+        // large values that has none. They go to fp16, whose eleven bits are more than those of q, the codes and the result; weights of
+        // more bits would need a second product. kLift puts the largest just below 2^15, so that all eleven are there down to 2^-29 of
+        // it and what is dropped is below 2^-40: where a key that has no value takes nearly all the weight, the others are the result.
         const float e_mine = vs > 0.0f ? float(min(ilogbf(vs), 127) + 1) : 0.0f;
         const float frac = vs > 0.0f ? ldexpf(vs, -int(e_mine)) : vs;
         float top[NT][2];
@@ -324,7 +327,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         }
         float top_v[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) top_v[n][0] = top[n][0] + e_mine, top_v[n][1] = top[n][1] + e_mine;
+        for (int n = 0; n < NT; ++n) top_v[n][0] = __fadd_ru(top[n][0], e_mine - kLift), top_v[n][1] = __fadd_ru(top[n][1], e_mine - kLift);  // no weight above 2^15
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1)
 #pragma unroll
@@ -458,7 +461,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sh_o[(warp * kKvHeadDim + d * 16 + gq + (e >> 1) * 8) * (kCols + 1) + n * 8 + q * 2 + (e & 1)] = o[d][n][e];
+          for (int e = 0; e < 4; ++e) sh_o[(warp * kKvHeadDim + d * 16 + gq + (e >> 1) * 8) * (kCols + 1) + n * 8 + q * 2 + (e & 1)] = o[d][n][e] * kLower;
       if (gq == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
           if (sh_seen[w][col] == 0) continue;
           const float ref = mm == -INFINITY ? 0.0f : mm;
           ll = fmaf(sh_l[w][col], sh_m[w][col] == -INFINITY && sh_l[w][col] == 0.0f ? 0.0f : exp2_fast(sh_m[w][col] - ref), ll);
-          const float f = sh_mv[w][col] == -INFINITY ? 1.0f : exp2_fast(sh_mv[w][col] - ref);  // a part without a finite score is 0 or NaN
+          const float f = sh_mv[w][col] == -INFINITY ? 1.0f : exp2_fast(sh_mv[w][col] - ref + kLift);  // a part without a finite score is 0 or NaN
 #pragma unroll
           for (int k = 0; k < 4; ++k) sum[k] = fmaf(sh_o[(w * kKvHeadDim + d4 + k) * (kCols + 1) + col], f, sum[k]);
         }

@@ -736,3 +736,44 @@ def test_heads_and_tokens_stand_for_themselves(news, group):
             got = c.cache.attention(c.seqs, other, c.heads).view(-1, 8, group, D)
             got[:, :, seed % group] = clean[:, :, seed % group]
             assert torch.equal(got, clean), (seed, bad, int((got != clean).sum()))
+
+
+@pytest.mark.parametrize("octaves", [14.7, 18.3, 22.3, 24.5, 25.5, 28.6])
+@pytest.mark.parametrize("news,group,n", [(1, 5, 700), (3, 4, 700), (6, 4, 700), (1, 4, 20000)])
+def test_a_key_that_takes_the_weight_and_has_no_value(octaves, news, group, n):
+    """The first key has nearly all the weight, and its value is zero: the output is what the others leave, each of them 2^-octaves of
+    the first one's weight. The bound is the file's: every weight is good to 2^-11 of itself."""
+    c = Case([news], [n], 1, group, 64, seed=81).fill([n])
+    page = c.table[0, : -(-n // 64)].long()
+    c.cache.k[page] = 0
+    c.cache.k[page[0], 0, 0, 0] = torch.tensor(1.0).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    c.cache.v[page] &= 0x7F  # magnitudes
+    c.cache.v[page[0], 0, :, 0] = 0
+    c.k.zero_()
+    c.k[0, 0, 0, 0] = float(c.cache.k_scale[page[0], 0])
+    c.v.abs_()
+    c.v[0, 0, 0] = 0
+    q = torch.zeros_like(c.q())
+    q.view(-1, group, D)[..., 0] = 1.0
+    c.check_attention(q, scale=octaves * math.log(2) / float(c.k[0, 0, 0, 0]))
+
+
+def test_values_near_the_smallest_scale():
+    """The same weights over values 2^-90 as large give a result 2^-90 as large, though it comes from small weights: the key that has
+    all but 2^-8 of the weight has no value, and each of the others 2^-18 of its weight. All values are positive: a rounding of each
+    result, and as much for the weights."""
+    n = 900
+    c = Case([1], [n], 1, 4, 16, seed=84).fill([n])
+    page = c.table[0, : -(-n // 16)].long()
+    c.cache.k[page] = 0
+    c.cache.k_scale[page] = 1.0
+    c.cache.k[page[3], 0, 9, 0] = 0x38  # 1.0
+    c.cache.v[page] &= 0x7F
+    c.cache.v[page[3], 0, :, 9] = 0
+    q = torch.zeros((1, 4 * D), dtype=torch.bfloat16, device="cuda")
+    q[0, ::D] = 1.0
+    c.cache.v_scale[page] = 2.0 ** -7
+    want = c.cache.attention(c.seqs, q, 4, scale=18 * math.log(2)).double()
+    c.cache.v_scale[page] = 2.0 ** -97
+    got = c.cache.attention(c.seqs, q, 4, scale=18 * math.log(2)).double() * 2.0 ** 90
+    assert float(want.min()) > 0 and bool(((got - want).abs() <= 2.0 ** -7 * want).all())
