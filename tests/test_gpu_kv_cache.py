@@ -777,3 +777,44 @@ def test_values_near_the_smallest_scale():
     c.cache.v_scale[page] = 2.0 ** -97
     got = c.cache.attention(c.seqs, q, 4, scale=18 * math.log(2)).double() * 2.0 ** 90
     assert float(want.min()) > 0 and bool(((got - want).abs() <= 2.0 ** -7 * want).all())
+
+
+@pytest.mark.parametrize("counts,past", [([1, 0, 1, 1], [0, 5, 63, 64]), ([5, 0, 16, 1], [0, 5, 60, 64]), ([5, 0, 40, 130], [0, 5, 60, 63])])
+def test_append_writes_no_row_or_column_beyond_its_own(counts, past):
+    """A q_out of its own, wider than the heads and longer than the sequences' rows, in each form of the launch: what is written is what a
+    plain call gives, and the rest of the buffer keeps what it held."""
+    lens = [a + b for a, b in zip(counts, past)]
+    c, d = (Case(counts, lens, 2, 3, 64, seed=91).fill(past) for _ in range(2))
+    qkv = new_qkv(c, extra=7)
+    cos, sin = tables(max(lens), 48, 5)
+    norms = (1 + 0.1 * torch.randn((2, D), device="cuda", generator=gen(6))).to(torch.bfloat16)
+    rotary = Rotary(cos, sin, None, norms[0], norms[1])
+    buffer = torch.full((c.rows + 7, c.heads * D + 24), -9.0, dtype=torch.bfloat16, device="cuda")
+    q = c.cache.append(c.seqs, qkv, c.heads, q_out=buffer[:, 8: 8 + c.heads * D], rotary=rotary)
+    rows = qkv[: c.rows].view(c.rows, -1, D)[:, : c.heads]
+    at = torch.cat([torch.arange(p, n, device="cuda") for p, n in zip(past, lens)])
+    want, mag = turned(rows, norms[0], cos, sin, at, rotary.eps)
+    got = q[: c.rows].reshape(c.rows, c.heads, D).double()
+    assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * mag + 1e-38).all())
+    keep = buffer.clone()
+    keep[: c.rows, 8: 8 + c.heads * D] = -9.0
+    assert bool((keep == -9.0).all())
+    assert torch.equal(d.cache.append(d.seqs, qkv, d.heads, rotary=rotary)[: c.rows], q[: c.rows])
+    for name in ("k", "v"):
+        assert torch.equal(getattr(c.cache, name), getattr(d.cache, name))
+    assert sfq.device_status() == 0
+
+
+def test_a_position_outside_the_tables_stands_for_the_first():
+    """It is reported, and the token is stored as if it stood at position 0."""
+    counts, lens = [1, 6], [9, 30]
+    c, d = (Case(counts, lens, 2, 2, 16, seed=92).fill([8, 24]) for _ in range(2))
+    qkv = new_qkv(c)
+    cos, sin = tables(50, 48, 7)
+    good = torch.tensor([4, 0, 2, 0, 49, 0, 7], dtype=torch.int32, device="cuda")
+    bad = torch.tensor([4, -1, 2, 50, 49, -(1 << 31), 7], dtype=torch.int32, device="cuda")
+    q = c.cache.append(c.seqs, qkv, 4, rotary=Rotary(cos, sin, good))
+    assert sfq.device_status() == 0
+    r = d.cache.append(d.seqs, qkv, 4, rotary=Rotary(cos, sin, bad))
+    assert sfq.device_status() == 42
+    assert torch.equal(q, r) and all(torch.equal(getattr(c.cache, n), getattr(d.cache, n)) for n in ("k", "v"))

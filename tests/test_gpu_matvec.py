@@ -221,3 +221,80 @@ def test_reads_behind_a_producer_and_writes_for_a_consumer():
         sfq.linear_matvec(w.desc, x, y)
         got.append(y.clone())
     assert all(torch.equal(g, wants[i % 4]) for i, g in enumerate(got))
+
+
+# Teams that take several groups of weight rows: the ring of copies that runs on into the next group, the next group's absmax, sums whose
+# place is used again, and with SwiGLU and odd remainders the rows past the end in the last group. On 148 SMs the first NVFP4 shape has
+# three rounds in every form, the others two.
+MANY = [("nvfp4", 40064, 192), ("nvfp4", 20096, 1088), ("nf4", 30018, 192), ("nf4", 20034, 1088), ("nf4", 9502, 2048)]
+
+
+@pytest.mark.parametrize("fmt,n,k", MANY)
+@pytest.mark.parametrize("rows", [1, 3, 4, 5, 8, 12, 16])
+@pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
+def test_teams_with_several_groups_of_rows(fmt, n, k, rows, act):
+    bias = {"none": None, "gelu": torch.float32, "swiglu": torch.bfloat16}[act]
+    check(Weight(fmt, n, k, n + rows, bias), draw_x(rows, k, rows) * (0.05 if fmt == "nvfp4" else 0.5), act)
+
+
+def spanning(x, where):
+    """x with elements over 100 binades in a part of K (fractions of it), and none but zeros in another."""
+    x, k = x.float(), x.shape[1]
+    a, b, c, d = (int(f * k) for f in where)
+    x[:, a:b] *= torch.exp2(torch.linspace(-60, 40, b - a, device="cuda"))
+    x[:, c:d] = 0
+    return x.to(torch.bfloat16)
+
+
+PARTS = [(0.0, 0.2, 0.5, 0.75), (0.8, 1.0, 0.0, 0.5), (0.3, 0.45, 0.0, 0.0), (0.0, 1.0, 0.0, 0.0)]
+
+
+@pytest.mark.parametrize("fmt,n,k", [("nvfp4", 40064, 192), ("nf4", 20034, 1088)])
+@pytest.mark.parametrize("rows", [1, 5, 12])
+@pytest.mark.parametrize("where", PARTS)
+def test_wide_x_through_several_groups_of_rows(fmt, n, k, rows, where):
+    """Every group is walked once for each band of 32 binades."""
+    check(Weight(fmt, n, k, n + rows), spanning(draw_x(rows, k, rows), where), "none")
+
+
+# K divided over clusters, of two CTAs and (514 rows) of four; all but 514 and 2432 rows with several groups for a team.
+CLUSTERS = [("nvfp4", 10240, 13824, 16), ("nvfp4", 2432, 13824, 13), ("nf4", 10274, 5120, 16), ("nf4", 514, 13824, 16), ("nf4", 5122, 13824, 5)]
+
+
+@pytest.mark.parametrize("fmt,n,k,rows", CLUSTERS)
+@pytest.mark.parametrize("act", ["none", "gelu", "swiglu"])
+@pytest.mark.parametrize("bias", [torch.float32, torch.bfloat16])
+def test_activations_and_bias_over_clusters(fmt, n, k, rows, act, bias):
+    check(Weight(fmt, n, k, n, bias), draw_x(rows, k, rows) * (0.01 if fmt == "nvfp4" else 0.1), act)
+
+
+@pytest.mark.parametrize("fmt,n,k,rows", CLUSTERS)
+@pytest.mark.parametrize("where", PARTS)
+def test_wide_x_over_clusters(fmt, n, k, rows, where):
+    """The CTAs of a cluster find different exponents and different numbers of bands in their parts of K, some of them none."""
+    x = spanning(draw_x(rows, k, rows), where)
+    x[rows // 2] = draw_x(1, k, 99)  # and a row within one band beside them
+    check(Weight(fmt, n, k, n), x)
+
+
+@pytest.mark.parametrize("fmt,n,k,rows", [("nvfp4", 128, 200000, 2), ("nf4", 66, 200000, 2), ("nf4", 2402, 123008, 1)])
+def test_the_largest_inputs(fmt, n, k, rows):
+    """Rows of x that only the shared memory of four CTAs holds."""
+    w = Weight(fmt, n, k, n)
+    check(w, draw_x(rows, k, rows))
+    check(w, spanning(draw_x(rows, k, rows), PARTS[1]))
+    with pytest.raises(sfq.SfqError, match="too large"):
+        big = sfq.QuantWeight.from_buffer_copy(w.desc)
+        big.in_features = 1 << 20
+        sfq.linear_matvec(big, torch.zeros((1, 1 << 20), dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "nf4"])
+@pytest.mark.parametrize("rows", [1, 4, 8, 16])
+@pytest.mark.parametrize("gate,up", [(1.0, 1.0), (0.2, 0.1), (6.0, 6.0)])
+def test_the_output_of_swiglu_as_input(fmt, rows, gate, up):
+    """What a down-projection is given, over many binades: silu(g) u in bf16. With deviations of 6 most rows need a second band."""
+    k = 6912
+    g = torch.Generator("cuda").manual_seed(rows)
+    a, b = (s * torch.randn((rows, k), device="cuda", generator=g) for s in (gate, up))
+    check(Weight(fmt, 1280, k, rows), (a * torch.sigmoid(a) * b).to(torch.bfloat16))
