@@ -392,7 +392,7 @@ void kv_append(KvCacheView c, int head_dim, const RotaryArgs& rot, const AppendA
       (g.heads > 0 && (g.ld_q < g.heads * kKvHeadDim || g.ld_q_out < g.heads * kKvHeadDim || g.ld_q % 8 != 0 || g.ld_q_out % 8 != 0 || !aligned16(g.q) || !aligned16(g.q_out))))
     throw std::invalid_argument("kv append: row pitches must cover heads * 128 columns and keep 16-byte alignment");
   const int q_cols = g.heads * kKvHeadDim, kv_cols = c.kv_heads * kKvHeadDim;
-  if (g.heads > 0 && ((!(g.q == g.q_out && g.ld_q == g.ld_q_out) && rows_overlap(g.q, g.ld_q, q_cols, g.q_out, g.ld_q_out, q_cols, c.rows)) ||
+  if (g.heads > 0 && ((!(g.q == g.q_out && (g.ld_q == g.ld_q_out || c.rows == 1)) && rows_overlap(g.q, g.ld_q, q_cols, g.q_out, g.ld_q_out, q_cols, c.rows)) ||
                       rows_overlap(g.k, g.ld_kv, kv_cols, g.q_out, g.ld_q_out, q_cols, c.rows) || rows_overlap(g.v, g.ld_kv, kv_cols, g.q_out, g.ld_q_out, q_cols, c.rows)))
     throw std::invalid_argument("kv append: q_out is q itself, with its pitch, or lies apart from q, k and v");
   if ((rot.cos == nullptr) != (rot.sin == nullptr)) throw std::invalid_argument("kv append: cos and sin come together");

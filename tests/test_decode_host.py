@@ -309,3 +309,11 @@ def test_pools_that_share_memory_are_refused():
             KvCache(*bad)
     scales = torch.zeros(20)
     KvCache(cache.k, cache.v, scales[10:].view(5, 2), scales[:10].view(5, 2))  # side by side
+
+
+def test_a_single_row_may_be_turned_in_place_with_any_pitch():
+    bad = sfq.RotaryDesc(d_cos=A, d_sin=A, table_rows=5, rotary_dim=24)  # the check behind that of the operands
+    fused = dict(q=A, ld_q=1024, q_out=A, ld_q_out=512, k=A + 512 * 2, v=A + 768 * 2, ld_kv=1024)
+    assert _append(_cache(), bad, **fused, rows=1) == sfq.ERR_INVALID_ARGUMENT and b"rotary_dim" in sfq.lib.sfq_last_error()
+    assert _append(_cache(), bad, **fused, rows=2) == sfq.ERR_INVALID_ARGUMENT and b"apart" in sfq.lib.sfq_last_error()
+    assert _append(_cache(), bad, **{**fused, "q_out": A + 16}, rows=1) == sfq.ERR_INVALID_ARGUMENT and b"apart" in sfq.lib.sfq_last_error()

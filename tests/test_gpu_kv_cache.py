@@ -818,3 +818,17 @@ def test_a_position_outside_the_tables_stands_for_the_first():
     r = d.cache.append(d.seqs, qkv, 4, rotary=Rotary(cos, sin, bad))
     assert sfq.device_status() == 42
     assert torch.equal(q, r) and all(torch.equal(getattr(c.cache, n), getattr(d.cache, n)) for n in ("k", "v"))
+
+
+@pytest.mark.parametrize("pad", [0, 64, 10])
+def test_one_token_in_place(pad):
+    c = Case([1], [70], 2, 3, 64, seed=93).fill([69])
+    d = Case([1], [70], 2, 3, 64, seed=93).fill([69])
+    qkv = new_qkv(c)
+    wide = torch.full((2, 10 * D + pad), 5.0, dtype=torch.bfloat16, device="cuda")
+    wide[0, : 10 * D] = qkv[0]
+    cos, sin = tables(70, 64, 8)
+    q = c.cache.append(c.seqs, wide[:1, : 10 * D], 6, q_out=wide[:1, : 6 * D], rotary=Rotary(cos, sin))
+    assert q.data_ptr() == wide.data_ptr() and torch.equal(q, d.cache.append(d.seqs, qkv, 6, rotary=Rotary(cos, sin)))
+    assert torch.equal(wide[0, 6 * D: 10 * D], qkv[0, 6 * D:]) and bool((wide[1] == 5).all()) and bool((wide[0, 10 * D:] == 5).all())
+    assert torch.equal(c.cache.k, d.cache.k) and torch.equal(c.cache.v, d.cache.v)
