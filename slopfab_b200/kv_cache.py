@@ -8,7 +8,7 @@ from dataclasses import dataclass
 import torch
 
 from . import KvCacheDesc, RotaryDesc, check, lib, ptr
-from .linear import on_device, raw_stream
+from .linear import SAME_DEVICE, on_device, raw_stream
 
 HEAD_DIM = 128
 _INT = torch.int32
@@ -126,22 +126,25 @@ class KvCache:
         return KvCacheDesc.from_buffer_copy(_FIELDS.pack(*pool, t.data_ptr(), n.data_ptr(), r.data_ptr(), batch, max_pages, s.max_new, s.max_len))
 
     def _pitch(self, name: str, t: torch.Tensor, rows: int | None, cols: int) -> int:
+        return self._rows_and_pitch(name, t, rows, cols)[1]
+
+    def _rows_and_pitch(self, name: str, t: torch.Tensor, rows: int | None, cols: int) -> tuple[int, int]:
         shape, stride = t.shape, t.stride()
         if t.dtype != torch.bfloat16 or len(shape) != 2 or shape[1] != cols or stride[1] != 1 or t.get_device() != self._device or rows not in (None, shape[0]):
             raise ValueError(f"{name} must be bf16 [{'rows' if rows is None else rows}, {cols}] with contiguous rows, on the cache's device")
         if shape[0] <= 1:
-            return cols  # a single row may have any stride
+            return shape[0], cols  # a single row may have any stride
         if stride[0] < cols:
             raise ValueError(f"{name}'s rows overlap: they lie {stride[0]} elements apart and have {cols}")
         if stride[0] >= 1 << 31:
             raise ValueError(f"{name}'s rows lie {stride[0]} elements apart; the library takes a pitch of 32 bits")
-        return stride[0]
+        return shape[0], stride[0]
 
     def append(self, s: Sequences, qkv: torch.Tensor, heads: int, q_out: torch.Tensor | None = None, rotary: Rotary | None = None) -> torch.Tensor:
         """Stores k and v of the fused projection qkv [rows, (heads + 2 kv_heads) * 128] and returns q, normed and rotated
         (q_out [rows, heads * 128]; pass a view of qkv's first columns to have it in place)."""
         pool = self._pool_now()
-        ld, rows = self._pitch("qkv", qkv, None, (heads + 2 * self.kv_heads) * HEAD_DIM), qkv.shape[0]
+        rows, ld = self._rows_and_pitch("qkv", qkv, None, (heads + 2 * self.kv_heads) * HEAD_DIM)
         ld_out = heads * HEAD_DIM
         if q_out is None:
             q_out = qkv.new_empty((rows, ld_out))
@@ -156,9 +159,14 @@ class KvCache:
                 raise ValueError("the rotation's tensors lie on the cache's device")
         q = qkv.data_ptr()
         k = q + heads * HEAD_DIM * 2
-        with on_device(self._device):
-            status = lib.sfq_kv_cache_append(C.byref(self._desc(s, pool)), C.byref(rotation) if rotation is not None else None, q, ld, q_out.data_ptr(), ld_out,
-                                             heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, raw_stream(self._device))
+        here = on_device(self._device)
+        args = (C.byref(self._desc(s, pool)), C.byref(rotation) if rotation is not None else None, q, ld, q_out.data_ptr(), ld_out,
+                heads, k, k + self.kv_heads * HEAD_DIM * 2, ld, rows, raw_stream(self._device))
+        if here is SAME_DEVICE:
+            status = lib.sfq_kv_cache_append(*args)
+        else:
+            with here:
+                status = lib.sfq_kv_cache_append(*args)
         if status:
             check(status)
         return q_out
@@ -167,7 +175,7 @@ class KvCache:
         """softmax(q K^T scale) V of the new tokens' q [rows, heads * 128] over the cache, causal among them; scale 0 means 1 / sqrt(128).
         The workspace is the call's own, so that calls on several streams and captured graphs share none."""
         pool = self._pool_now()
-        ld, rows = self._pitch("q", q, None, heads * HEAD_DIM), q.shape[0]
+        rows, ld = self._rows_and_pitch("q", q, None, heads * HEAD_DIM)
         ld_out = heads * HEAD_DIM
         if out is None:
             out = q.new_empty((rows, ld_out))

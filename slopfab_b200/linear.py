@@ -24,10 +24,10 @@ def on_device(index: int):
     """Makes device `index` current for a call, at no cost where it is already."""
     if index < 0:
         raise ValueError("tensors must be on a CUDA device")
-    return _SAME if index == _current_device() else torch.cuda.device(index)
+    return SAME_DEVICE if index == _current_device() else torch.cuda.device(index)
 
 
-_SAME = contextlib.nullcontext()
+SAME_DEVICE = contextlib.nullcontext()
 _current_device = torch._C._cuda_getDevice  # without a look whether CUDA is up: a tensor lies on it
 raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device, without the Python object
 
