@@ -436,11 +436,12 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
         for (int e = 0; e < 4; ++e) part((warp * MT * 16 + m * 16 + gq + (e >> 1) * 8) * kPitch + n * 8 + q * 2 + (e & 1)) = acc[m][n][e];
     named_barrier(team + 1, kTeamWarps * 32);
   };
+  int map_e = 0;  // NF4: exponent that the table is over
   auto summed = [&](int r, int row) {  // the team's sum of a row of the tiles and a row of x
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < kTeamWarps; ++w) s += part((w * MT * 16 + row) * kPitch + r);
-    return ldexpf(s * g.global_scale, row_e[r] - 14);
+    return ldexpf(s * g.global_scale, row_e[r] - 14 + map_e);
   };
   auto bias_of = [&](int at) {
     return g.bias == nullptr ? 0.0f : g.bias_is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g.bias)[at]) : static_cast<const float*>(g.bias)[at];
@@ -490,10 +491,14 @@ __global__ void __launch_bounds__(WARPS * 32, (!NF4 && D == 4) ? 2 : 1) matvec_k
   const float map = NF4 ? g.map[lane & 15] : 0.0f, nested = NF4 ? g.nested_map[threadIdx.x & 255] : 0.0f;
   const bool misfit = stage_x(-1);
   if constexpr (NF4) {
-    // the table: the entry of a byte, odd element (low nibble) in the low half, and its 32 copies
+    // the table: the entry of a byte, odd element (low nibble) in the low half, and its 32 copies. Entries are over the exponent of the
+    // largest finite one, so that a map of any size is as good in fp16.
+    const uint32_t size = __float_as_uint(map) & 0x7FFFFFFFu, top = __reduce_max_sync(0xffffffffu, size < 0x7F800000u ? size : 0u);
+    map_e = top == 0 ? 0 : max(int(top >> 23), 1) - 127;
+    const float even = ldexpf(map, -map_e);
     for (uint32_t i = threadIdx.x; i < 256 * 8; i += kThreads) {  // whole warps
       const uint32_t b = i >> 3;
-      const __half2 pair = __floats2half2_rn(__shfl_sync(0xffffffffu, map, b & 15), __shfl_sync(0xffffffffu, map, b >> 4));
+      const __half2 pair = __floats2half2_rn(__shfl_sync(0xffffffffu, even, b & 15), __shfl_sync(0xffffffffu, even, b >> 4));
       const uint32_t v = *reinterpret_cast<const uint32_t*>(&pair);
       *reinterpret_cast<uint4*>(smem + b * 256 + (i & 7) * 16) = make_uint4(v, v, v, v);
     }

@@ -298,3 +298,16 @@ def test_the_output_of_swiglu_as_input(fmt, rows, gate, up):
     g = torch.Generator("cuda").manual_seed(rows)
     a, b = (s * torch.randn((rows, k), device="cuda", generator=g) for s in (gate, up))
     check(Weight(fmt, 1280, k, rows), (a * torch.sigmoid(a) * b).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 16])
+@pytest.mark.parametrize("size", [-100, -30, -16, 17, 60])
+def test_nf4_maps_of_every_size(rows, size):
+    """A map 2^size as large over an absmax 2^-size as large is the same weight, and gives the same bits."""
+    w = Weight("nf4", 130, 640, 12, torch.float32)
+    x = draw_x(rows, 640, rows)
+    want = check(w, x, "gelu")
+    w.map *= 2.0 ** size
+    w.nested_absmax *= 2.0 ** -size
+    w.desc.nf4_nested_offset *= 2.0 ** -size
+    assert torch.equal(check(w, x, "gelu"), want)
