@@ -462,9 +462,13 @@ SFQ_API int sfq_attention_forward(const void* d_q_bf16, int ld_q, const void* d_
 /* y[rows, out] = act(x[rows, in] W^T + b) for few rows, without a dense copy of the weight and with bf16 activations: W is what the
  * stored bytes say (code x group scale x tensor scale, not rounded to bf16), sums are fp32, the result is rounded once. Formats: SFQ_NVFP4
  * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 64 == 0, block sizes powers of two, of 64 elements at least; the 16
- * table entries are rounded to fp16); no AWQ pre-scale, no ConvRot; in up to 200000.
+ * table entries are rounded to fp16 over the exponent of the largest: eleven bits down to 2^-14 of it); no AWQ pre-scale, no ConvRot; in up to 200000, and where the device cannot schedule clusters of
+ * four such CTAs up to 91648 (NVFP4) and 65536 (NF4).
  * activation: sfq_activation; SFQ_ACT_SWIGLU takes [gate | up] rows (any even out) and writes out / 2 columns. Any number of rows; the
- * weight is read once for 16 of them. x and the weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
+ * weight is read once for 16 of them up to in 10240 (NVFP4) and 7424 (NF4), twice that where out <= 2368, and beyond once for as many as
+ * the shared memory of a cluster takes of x. A call whose x has an element other than zero below 2^-23 or from 1024 up looks at x again and
+ * takes two to three times as long; where a row of x spans more than 32 binades the weight is gone through once for each 32 of them, too. x and the
+ * weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
 SFQ_API int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, int rows, int activation, void* d_y_bf16, void* stream);
 
 /* Keys and values of many sequences in pages of `page_size` tokens, 8 bits a value: e4m3 codes, K as [num_pages, kv_heads, page_size, 128]
@@ -474,7 +478,8 @@ SFQ_API int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, i
  * tokens (none: an empty range); rows behind the last sequence's are left as they were. max_new and max_len are the host's estimates of
  * the most new tokens and the longest sequence: they size the launch, no result depends on them beyond the order of fp32 sums.
  * Entries that make no sense are not followed: the tokens they would address are skipped, and sfq_device_status reports 40 (row
- * starts or a length), 41 (a page outside the pool) or 42 (a rotation position outside the tables). */
+ * starts or a length) or 41 (a page outside the pool). A rotation position outside the tables stands for the tables' first row, and
+ * sfq_device_status reports 42. */
 typedef struct sfq_kv_cache {
   void* d_k;
   void* d_v;
@@ -508,7 +513,7 @@ typedef struct sfq_rotary {
 } sfq_rotary;
 
 /* Puts the new tokens' k and v [rows, kv_heads * 128] into their pages and writes q [rows, heads * 128] normed and rotated to d_q_out
- * (d_q itself with its pitch, or apart from q, k and v; heads 0: no q). The scale of a (page, head) is the smallest power of two s (2^-100 at least) with |x| <= 448 s over
+ * (d_q itself with its pitch, which for one row may be any, or apart from q, k and v; heads 0: no q). The scale of a (page, head) is the smallest power of two s (2^-100 at least) with |x| <= 448 s over
  * the finite values put there so far; a first token in a page starts it anew, a later one can only raise it, and the codes that are there
  * are then rounded again. Infinities are stored as +-448 s, NaN as NaN. `rotary` may be null. A page that is being written
  * belongs to one sequence and stands once in its row of the table. */

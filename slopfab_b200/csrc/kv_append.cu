@@ -222,8 +222,8 @@ __global__ void __launch_bounds__(128) kv_append_few_kernel(KvCacheView c, Rotar
 
 // Several tokens, prompts. blockIdx.x: a kv head, behind them groups of query heads; y: sequence; z: page of the sequence's new tokens, so that what runs at
 // a time reads rows of a fused projection whole (with the pages first 38.6 us in place of 36.3). A thread takes the
-// same piece of up to kHeld tokens' vectors, which stay in registers while the block finds the page's scale (pages of more than 64 tokens
-// are computed twice); V goes through shared memory, so that a channel's tokens are stored side by side.
+// same piece of up to kHeld tokens' vectors, which stay in registers while the block finds the page's scale (more than 64 tokens of a
+// page, 16 with 128 threads, are computed twice); V goes through shared memory, so that a channel's tokens are stored side by side.
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) kv_append_page_kernel(KvCacheView c, RotaryArgs rot, AppendArgs g) {
   constexpr int kAtOnce = kThreads / kLanes;  // vectors a block works on at once
