@@ -218,15 +218,16 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = max(int(top >> 7), 1) - 127;  // exponent of the largest element
-        const float up = ldexpf(1.0f, min(14 - e, 127)), up2 = ldexpf(1.0f, 14 - e - min(14 - e, 127));
+        // Exponent of the largest element, -108 at least: bf16's smallest number is then still a normal fp16, and so is the factor of the scores.
+        const int e = max(int(top >> 7) - 127, -108);
+        const float up = ldexpf(1.0f, 14 - e);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint32_t w[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t r = raw[2 * j + h];
-            w[h] = half_pair(__uint_as_float(r << 16) * up * up2, __uint_as_float(r & 0xFFFF0000u) * up * up2);
+            w[h] = half_pair(__uint_as_float(r << 16) * up, __uint_as_float(r & 0xFFFF0000u) * up);
           }
           sh_q[j][col >> 3][(col & 7) * 4 + quarter] = make_uint2(w[0], w[1]);
         }

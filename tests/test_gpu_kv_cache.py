@@ -832,3 +832,14 @@ def test_one_token_in_place(pad):
     assert q.data_ptr() == wide.data_ptr() and torch.equal(q, d.cache.append(d.seqs, qkv, 6, rotary=Rotary(cos, sin)))
     assert torch.equal(wide[0, 6 * D: 10 * D], qkv[0, 6 * D:]) and bool((wide[1] == 5).all()) and bool((wide[0, 10 * D:] == 5).all())
     assert torch.equal(c.cache.k, d.cache.k) and torch.equal(c.cache.v, d.cache.v)
+
+
+@pytest.mark.parametrize("shift", [-130, -128, -126, -124])
+def test_the_smallest_queries_over_the_largest_keys(shift):
+    """Scores of an ordinary size from queries near the end of bf16's range and keys near the other end of the scales'."""
+    c = Case([1], [300], 1, 4, 64, seed=94).fill([300])
+    c.cache.k_scale *= 2.0 ** 125
+    c.k *= 2.0 ** 125
+    q = (c.q().clamp(-4, 4).double() * 2.0 ** shift).to(torch.bfloat16)
+    c.check_attention(q)
+    c.check_attention(q, scale=0.3)
