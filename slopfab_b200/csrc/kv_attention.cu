@@ -307,8 +307,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         // more bits would need a second product (two fp16 terms: 46.9, 55.0 and 59.3 us where one term takes 42.8, 53.4 and 52.8, and
         // the results' distance from 64 bits stays 1.67e-3 of their norm, the rounding to bf16). kLift puts the largest just below 2^15, so that all eleven are there down to 2^-29 of
         // it and what is dropped is below 2^-40: where a key that has no value takes nearly all the weight, the others are the result.
-        const float e_mine = vs > 0.0f ? float(min(ilogbf(vs), 127) + 1) : 0.0f;
-        const float frac = vs > 0.0f ? ldexpf(vs, -int(e_mine)) : vs;
+        const float e_mine = fabsf(vs) > 0.0f ? float(min(ilogbf(vs), 127) + 1) : 0.0f;
+        const float frac = fabsf(vs) > 0.0f ? ldexpf(vs, -int(e_mine)) : vs;
         float top[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {

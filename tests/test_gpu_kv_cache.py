@@ -843,3 +843,17 @@ def test_the_smallest_queries_over_the_largest_keys(shift):
     q = (c.q().clamp(-4, 4).double() * 2.0 ** shift).to(torch.bfloat16)
     c.check_attention(q)
     c.check_attention(q, scale=0.3)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -9, 1.0, 4.0, 2.0 ** 40])
+def test_negative_scales(size):
+    """A page whose scale of V, or of K, is negative stands for the negative of its codes' values."""
+    c = Case([2], [200], 2, 3, 32, seed=95).fill([200])
+    for name, t in (("v_scale", c.v), ("k_scale", c.k)):
+        for p in (0, 3, 6):
+            i = int(c.table[0, p])
+            was = getattr(c.cache, name)[i].clone()
+            now = -(torch.full_like(was, size) if name == "v_scale" else was)
+            t[0, :, 32 * p: 32 * p + 32] *= (now / was).double()[:, None, None]
+            getattr(c.cache, name)[i] = now
+        c.check_attention(c.q())
