@@ -461,14 +461,14 @@ SFQ_API int sfq_attention_forward(const void* d_q_bf16, int ld_q, const void* d_
 
 /* y[rows, out] = act(x[rows, in] W^T + b) for few rows, without a dense copy of the weight and with bf16 activations: W is what the
  * stored bytes say (code x group scale x tensor scale, not rounded to bf16), sums are fp32, the result is rounded once. Formats: SFQ_NVFP4
- * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 64 == 0, block sizes powers of two, of 64 elements at least; the 16
- * table entries are rounded to fp16 over the exponent of the largest: eleven bits down to 2^-14 of it); no AWQ pre-scale, no ConvRot; in up to 200000, and where the device cannot schedule clusters of
- * four such CTAs up to 91648 (NVFP4) and 65536 (NF4).
+ * (out % 128 == 0, in % 64 == 0) and SFQ_NF4 (in % 64 == 0, block sizes powers of two, of 64 elements at least; the 16 table entries are
+ * rounded to fp16 over the exponent of the largest: eleven bits down to 2^-14 of it); no AWQ pre-scale, no ConvRot; in up to 200000, and
+ * where the device cannot schedule clusters of four such CTAs up to 91648 (NVFP4) and 65536 (NF4).
  * activation: sfq_activation; SFQ_ACT_SWIGLU takes [gate | up] rows (any even out) and writes out / 2 columns. Any number of rows; the
  * weight is read once for 16 of them up to in 10240 (NVFP4) and 7424 (NF4), twice that where out <= 2368, and beyond once for as many as
- * the shared memory of a cluster takes of x. A call whose x has an element other than zero below 2^-23 or from 1024 up looks at x again and
- * takes two to three times as long; where a row of x spans more than 32 binades the weight is gone through once for each 32 of them, too. x and the
- * weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
+ * the shared memory of a cluster takes of x. A call whose x has an element other than zero below 2^-23 or from 1024 up looks at x again
+ * and takes two to three times as long; where a row of x spans more than 32 binades the weight is gone through once for each 32 of them,
+ * too. x and the weight bytes 16-byte aligned, x and y apart. rows <= 0 is a no-op. */
 SFQ_API int sfq_linear_matvec(const sfq_quant_weight* w, const void* d_x_bf16, int rows, int activation, void* d_y_bf16, void* stream);
 
 /* Keys and values of many sequences in pages of `page_size` tokens, 8 bits a value: e4m3 codes, K as [num_pages, kv_heads, page_size, 128]
@@ -513,19 +513,19 @@ typedef struct sfq_rotary {
 } sfq_rotary;
 
 /* Puts the new tokens' k and v [rows, kv_heads * 128] into their pages and writes q [rows, heads * 128] normed and rotated to d_q_out
- * (d_q itself with its pitch, which for one row may be any, or apart from q, k and v; heads 0: no q). The scale of a (page, head) is the smallest power of two s (2^-100 at least) with |x| <= 448 s over
- * the finite values put there so far; a first token in a page starts it anew, a later one can only raise it, and the codes that are there
- * are then rounded again. Infinities are stored as +-448 s, NaN as NaN. `rotary` may be null. A page that is being written
- * belongs to one sequence and stands once in its row of the table. */
+ * (d_q itself with its pitch, which for one row may be any, or apart from q, k and v; heads 0: no q). The scale of a (page, head) is the
+ * smallest power of two s (2^-100 at least) with |x| <= 448 s over the finite values put there so far; a first token in a page starts it
+ * anew, a later one can only raise it, and the codes that are there are then rounded again. Infinities are stored as +-448 s, NaN as NaN.
+ * `rotary` may be null. A page that is being written belongs to one sequence and stands once in its row of the table. */
 SFQ_API int sfq_kv_cache_append(const sfq_kv_cache* cache, const sfq_rotary* rotary, const void* d_q_bf16, int ld_q, void* d_q_out_bf16,
                                 int ld_q_out, int heads, const void* d_k_bf16, const void* d_v_bf16, int ld_kv, int rows, void* stream);
 
 /* out[rows, heads * 128] = softmax(q K^T scale) V over the cache: the i-th of a sequence's n new tokens sees its first length - n + i + 1
  * keys; query head h reads kv head h / (heads / kv_heads). scale <= 0 selects 1 / sqrt(128). out and q lie apart. A row that sees no key is zero; a NaN or +inf
- * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Scores, weights and sums are fp32; in front
- * of V a weight is rounded to fp16, relative to the largest weight near it: to eleven bits down to 2^-29 of that one, to zero below 2^-40. Slots behind a sequence's length may hold
- * anything. The workspace is scratch of one call and needs no initialisation; it may be null where
- * sfq_kv_cache_attention_workspace_bytes gives 0. */
+ * score makes its row NaN, a score of -inf has no weight, and a row without a finite score is NaN. Scores, weights and sums are fp32; in
+ * front of V a weight is rounded to fp16, relative to the largest weight near it: to eleven bits down to 2^-29 of that one, to zero below
+ * 2^-40. Slots behind a sequence's length may hold anything. The workspace is scratch of one call and needs no initialisation; it may be
+ * null where sfq_kv_cache_attention_workspace_bytes gives 0. */
 SFQ_API int sfq_kv_cache_attention_workspace_bytes(const sfq_kv_cache* cache, int heads, int rows, size_t* out);
 SFQ_API int sfq_kv_cache_attention(const sfq_kv_cache* cache, const void* d_q_bf16, int ld_q, void* d_out_bf16, int ld_out, int heads,
                                    int rows, float scale, void* d_workspace, size_t workspace_bytes, void* stream);

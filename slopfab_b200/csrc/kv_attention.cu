@@ -12,7 +12,7 @@
 // the weight.
 // Long sequences are divided over CTAs (flash decoding); a second launch joins their parts in order.
 // Measured in a graph, 40 query heads on 8 kv heads: one sequence of 333 tokens 8.7 us, of 131072 51.0 (5.3 TB/s), 32 of up to 4096
-// 42.4 (4.1 TB/s). 16 of up to 3001 with five new tokens, 40 heads on 10, 52.1 us: three query tiles of
+// 42.2 (4.1 TB/s). 16 of up to 3001 with five new tokens, 40 heads on 10, 52.0 us: three query tiles of
 // eight, where scores, exponentials and products, not memory, take the time. Prompts go through 24 query columns at a time, which is right
 // but not fast: 4747 new tokens, 40 heads on 10, 1.5 ms, behind as many cached ones 3.8.
 #include <cuda_fp16.h>
@@ -301,12 +301,13 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? kResident[NT] : 1) 
         // ---- weights
         const bool whole = __all_sync(0xffffffffu, page >= 0) && t0 + kTile <= min(first_hidden, length);
         const int mine = t0 + (gq >> 1) * 16 + (gq & 1);  // token of row gq of MMA 0; row gq + 8 is two behind, MMA t four t
-        // The weights of the second product are p vs = exp2(score + e) (vs / 2^e) with vs / 2^e in [0.5, 1), over their own running
+        // The weights of the second product are p vs = exp2(score + e) (vs / 2^e) with |vs| / 2^e in [0.5, 1), over their own running
         // reference mv, the largest score + e less kLift: a page of small values that has all the weight keeps its bits beside one of
-        // large values that has none. They go to fp16, whose eleven bits are more than those of q, the codes and the result; weights of
-        // more bits would need a second product (two fp16 terms: 46.9, 55.0 and 59.3 us where one term takes 42.8, 53.4 and 52.8, and
-        // the results' distance from 64 bits stays 1.67e-3 of their norm, the rounding to bf16). kLift puts the largest just below 2^15, so that all eleven are there down to 2^-29 of
-        // it and what is dropped is below 2^-40: where a key that has no value takes nearly all the weight, the others are the result.
+        // large values that has none. They go to fp16, whose eleven bits are more than those of q, the codes and the result. Weights of
+        // more bits would need a second product: with two fp16 terms 32 x 4096 takes 46.9 us in place of 42.8, 1 x 131072 55.0 and not
+        // 53.4, 16 x 5 new tokens 59.3 and not 52.8 (called), and the results stay 1.67e-3 of their norm from 64 bits, the rounding to
+        // bf16. kLift puts the largest just below 2^15, so that all eleven bits are there down to 2^-29 of it and what is dropped is below
+        // 2^-40: where a key that has no value takes nearly all the weight, the others are the result.
         const float e_mine = fabsf(vs) > 0.0f ? float(min(ilogbf(vs), 127) + 1) : 0.0f;
         const float frac = fabsf(vs) > 0.0f ? ldexpf(vs, -int(e_mine)) : vs;
         float top[NT][2];
